@@ -30,6 +30,10 @@ ARCH = "gfx950"
 CFLAGS = [
     "-O3", f"--offload-arch={ARCH}", "-fPIC", "-std=c++17", "-ffp-contract=off",
     "-fhip-fp32-correctly-rounded-divide-sqrt", "-Wall", "-Wno-unused-function",
+    # no packed fp32 instructions (two fp32 operations in one v_pk_*_f32): some of their forms
+    # have given wrong results on this hardware. The scalar forms round the same, so every
+    # result keeps its bits. (The host pass warns that it does not know the feature.)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # compressed code-object bundles (the HIP runtime inflates them at load): the library
     # goes from 9.4 to ~3.5 MB, which every GPU-box push carries
     "--offload-compress",
@@ -48,7 +52,8 @@ def sources() -> list[Path]:
 
 
 def _headers() -> list[Path]:
-    return sorted(list(CSRC.glob("*.h")) + list(INCLUDE.glob("*.h")))
+    # this file too: its flags change what every object holds
+    return sorted(list(CSRC.glob("*.h")) + list(INCLUDE.glob("*.h"))) + [Path(__file__).resolve()]
 
 
 def _stale(obj: Path, deps: list[Path]) -> bool:
