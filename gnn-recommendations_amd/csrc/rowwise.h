@@ -1,0 +1,122 @@
+// What the row-wise kernels share (dropout, layer norm, the 4-bit tables): element types, loads
+// and stores of eight neighbouring elements, and the dropout's counter-based generator.
+#pragma once
+
+#include "common.h"
+
+namespace gnnrec {
+
+// Tables of these kernels hold float, bfloat16 or half; all arithmetic is in 32 bits, and a
+// result is rounded once (to nearest, ties to even) when it is stored.
+using bf16_t = __bf16;
+using f16_t = _Float16;
+
+// Runs f(T{}) for the element type of a gnnrec_dtype value (already checked).
+template <class F>
+inline int with_dtype(int32_t t, F&& f) {
+  if (t == GNNREC_F32) return f(float{});
+  if (t == GNNREC_BF16) return f(bf16_t{});
+  return f(f16_t{});
+}
+inline bool dtype_ok(int32_t t) { return t == GNNREC_F32 || t == GNNREC_BF16 || t == GNNREC_F16; }
+
+// Eight neighbouring elements; aligned as one element only, so that rows of any width and
+// stride load with 16-B instructions (the hardware takes unaligned vector accesses).
+template <class T>
+struct __attribute__((packed)) Eight {
+  T v[8];
+};
+
+// v[e] = p[e] for e < n, 0 for the others. n >= 8: one vector access.
+template <class T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, int64_t n, float (&v)[8]) {
+  if (n >= 8) {
+    const Eight<T> t = *reinterpret_cast<const Eight<T>*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)t.v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.f;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T* __restrict__ p, int64_t n, const float (&v)[8]) {
+  if (n >= 8) {
+    Eight<T> t;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t.v[e] = (T)v[e];
+    *reinterpret_cast<Eight<T>*>(p) = t;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (T)v[e];
+  }
+}
+
+// ---- dropout ------------------------------------------------------------------------------
+// Philox4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy
+// as 1, 2, 3", 2011): a keyed bijection of a 128-bit counter. Here the key is the seed and the
+// counter (column / 8, row, site), so a block's 128 bits are the eight 16-bit draws of eight
+// neighbouring columns of a row. A value depends on its place alone: not on the launch, the
+// table's stride or the shard that holds the row, and the backward pass draws the same mask
+// again instead of reading it.
+struct Drop {
+  const int64_t* seed_ptr;  // the seed in device memory (a captured graph's), or NULL
+  uint64_t seed;
+  uint32_t site;
+  uint32_t border;  // a draw below it drops the value; 65536 drops all, 0 none
+  float scale;      // 65536 / (65536 - border): the expectation is kept for the border used
+  float slope;      // of the LeakyReLU in front (1: none)
+  int64_t row0;     // global row of the table's first one
+};
+
+__device__ __forceinline__ uint64_t drop_key(const Drop& d) {
+  return d.seed_ptr ? (uint64_t)*d.seed_ptr : d.seed;
+}
+
+__device__ __forceinline__ void philox(uint64_t key, uint32_t c0, uint64_t row, uint32_t site,
+                                       uint32_t (&w)[4]) {
+  uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
+  uint32_t x0 = c0, x1 = (uint32_t)row, x2 = (uint32_t)(row >> 32), x3 = site;
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const uint64_t a = (uint64_t)x0 * 0xD2511F53u, b = (uint64_t)x2 * 0xCD9E8D57u;
+    x0 = (uint32_t)(b >> 32) ^ x1 ^ k0;
+    x1 = (uint32_t)b;
+    x2 = (uint32_t)(a >> 32) ^ x3 ^ k1;
+    x3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  w[0] = x0, w[1] = x1, w[2] = x2, w[3] = x3;
+}
+
+// f[e] = scale where value e of block (row, cb) is kept, 0 where it is dropped.
+__device__ __forceinline__ void drop_factors(const Drop& d, uint64_t key, int64_t row, uint32_t cb,
+                                             float (&f)[8]) {
+  uint32_t w[4];
+  philox(key, cb, (uint64_t)(d.row0 + row), d.site, w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    f[e] = ((w[e >> 1] >> (16 * (e & 1))) & 0xffffu) >= d.border ? d.scale : 0.f;
+}
+
+// Fills a Drop from the C ABI's arguments; false (and the message set) if they are unusable.
+inline bool make_drop(Drop* d, const char* what, double p, uint64_t seed, const int64_t* seed_ptr,
+                      uint32_t site, int64_t row0, float slope) {
+  if (!(p >= 0.0 && p <= 1.0)) {
+    set_error("%s: p must be between 0 and 1, got %g", what, p);
+    return false;
+  }
+  if (row0 < 0) {
+    set_error("%s: negative row0", what);
+    return false;
+  }
+  const uint32_t border = (uint32_t)(p * 65536.0 + 0.5);
+  *d = Drop{seed_ptr, seed, site, border,
+            border < 65536 ? (float)(65536.0 / (65536 - border)) : 0.f, slope, row0};
+  return true;
+}
+
+}  // namespace gnnrec

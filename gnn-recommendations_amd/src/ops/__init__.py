@@ -20,10 +20,13 @@ from .graph import CsrGraph, ShardInfo, inv_sqrt_degrees
 from . import functional, library  # library: registers torch.ops.gnnrec.*
 from .functional import (dense_layer, gas, gat_aggregate, lightgcn_propagate, ngcf_layer,
                          score_topk, spmm, spmm_gas)
+from .rowwise import dropout, dropout_add_layer_norm, layer_norm
+from .q4 import Q4Table, q4_matmul, quantize_q4
 
 __all__ = ["CsrGraph", "ShardInfo", "inv_sqrt_degrees", "functional", "spmm", "spmm_gas",
            "gas", "ngcf_layer", "dense_layer", "gat_aggregate", "score_topk", "lightgcn_propagate", "as_operand",
-           "sparse_mm", "uses_native"]
+           "sparse_mm", "uses_native", "dropout", "layer_norm", "dropout_add_layer_norm",
+           "Q4Table", "quantize_q4", "q4_matmul"]
 
 _CACHE: dict = {}
 

@@ -13,12 +13,14 @@ import ctypes as C
 import os
 from pathlib import Path
 
-import torch  # noqa: F401  (load order: torch's HIP runtime first)
+import torch  # (load order: torch's HIP runtime first)
 
 _PKG_ROOT = Path(__file__).resolve().parents[2]
 LIB_PATH = Path(os.environ.get("GNNREC_LIB", _PKG_ROOT / "lib" / "libgnnrec.so"))
-ABI_VERSION = 11
+ABI_VERSION = 12
 
+# gnnrec.h gnnrec_dtype
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # gnnrec.h epilogue flags
 EPI_ACC_INIT = 1
 EPI_ACC_ADD = 2
@@ -47,6 +49,9 @@ TILED_MAX_CLASSES = 256
 TILED_MAX_ROWS_FACTORED = 1232
 
 _p = C.c_void_p
+_u32 = C.c_uint32
+_u64 = C.c_uint64
+_f64 = C.c_double
 _i64 = C.c_int64
 _i32 = C.c_int32
 _f32 = C.c_float
@@ -136,9 +141,23 @@ _SIGNATURES = {
     "gnnrec_normalize_values_device": [_p, _p, _p, _i64, _p, _i32, _p, _p],
     "gnnrec_adam_step_f32": [_p, _p, _p, _p, _i64, _f32, C.c_double, C.c_double, _f32, _f32,
                              _f32, _p, _p],
+    "gnnrec_dropout_forward": [_i32, _i64, _i64, _p, _i64, _p, _i64, _f64, _u64, _p, _u32, _i64,
+                               _f32, _p],
+    "gnnrec_dropout_backward": [_i32, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _f64, _u64, _p,
+                                _u32, _i64, _f32, _p],
+    "gnnrec_layer_norm_forward": [_i32, _i32, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _f32, _f64,
+                                  _u64, _p, _u32, _i64, _f32, _p, _i64, _p, _i64, _p],
+    "gnnrec_layer_norm_work_floats": [_i64, _i64],
+    "gnnrec_layer_norm_backward": [_i32, _i32, _i64, _i64, _p, _i64, _p, _i64, _p, _f32, _f64,
+                                   _u64, _p, _u32, _i64, _f32, _p, _i64, _p, _i64, _p, _i64, _p,
+                                   _i64, _p, _p, _p, _p],
+    "gnnrec_quantize_q4": [_i32, _i64, _i64, _p, _i64, _p, _p, _p],
+    "gnnrec_dequantize_q4": [_i64, _i64, _p, _p, _p, _i64, _p],
+    "gnnrec_q4_matmul": [_i32, _i32, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
 }
 _RESTYPES = {"gnnrec_version": C.c_char_p, "gnnrec_last_error": C.c_char_p,
-             "gnnrec_abi_version": C.c_int, "gnnrec_tiled_plan_device_scratch_words": C.c_int64}
+             "gnnrec_abi_version": C.c_int,
+             "gnnrec_layer_norm_work_floats": C.c_int64, "gnnrec_tiled_plan_device_scratch_words": C.c_int64}
 
 EXPORTED = tuple(_SIGNATURES)
 

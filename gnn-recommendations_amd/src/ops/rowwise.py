@@ -1,0 +1,239 @@
+"""Row-wise operators of the training path over libgnnrec: dropout from a counter-based
+generator, layer norm, and the block between two hops that joins them.
+
+    dropout(x, p, seed)                                  keep ? leaky(x) / (1 - p) : 0
+    layer_norm(x, weight, bias)                          (x - mean) / sqrt(var + eps) w + b
+    dropout_add_layer_norm(x, residual, weight, bias, p, seed)
+                                                         h = residual + dropout(leaky(x)); LN(h), h
+
+Tables on a ROCm device, fp32 / bf16 / fp16, 2-D row-major views with any row stride (0 too) or
+contiguous tensors of any rank (rows are the last dimension); launched on torch's current stream
+of the table's device. All differentiable (once), each backward pass one launch (two with a
+weight gradient) that repeats the forward's arithmetic from its inputs: no mask, statistics or
+normalised rows are kept.
+
+The dropout's mask: value (row, column) is dropped when its 16-bit draw is below
+round(p * 65536), the others are scaled by 65536 / (65536 - round(p * 65536)). The draws are
+Philox4x32-10 (Salmon et al., 2011) with key = `seed` and counter = (column // 8, row0 + row,
+site), so they depend on nothing else: a row shard that passes its first global row as `row0`
+draws what one device would, and a second dropout of the same step takes another `site`. `seed`
+is an int or a one-element int64 tensor on the table's device; a captured graph reads the tensor
+on every replay, so `seed.add_(1)` between replays (or captured in front) gives new masks.
+A dropped value is 0 whatever x holds there, also an infinity or a NaN.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import check, ptr
+
+MAX_NORM_WIDTH = 16384    # csrc/layer_norm.hip kNormMaxD
+
+Seed = Union[int, torch.Tensor]
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call a C entry on `device`'s current stream, whatever device is current."""
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, _lib.stream_of(device)), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _lib.stream_of(device)), name)
+
+
+def rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
+    """t as the 2-D [rows, width] view that the kernels take; raises where there is none."""
+    if not t.is_cuda:
+        raise ValueError(f"{what}: needs a tensor on a ROCm device, got {t.device}")
+    if t.dtype not in _lib.DTYPES:
+        raise TypeError(f"{what}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{what}: expected rows of at least one value, got {tuple(t.shape)}")
+    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1):
+        return t
+    if t.is_contiguous():
+        return t.view(-1, t.shape[-1])
+    raise ValueError(f"{what}: expected a 2-D row-major table (stride(1) == 1) or a contiguous "
+                     "tensor")
+
+
+def _rows_or_copy(t: torch.Tensor, what: str) -> torch.Tensor:
+    """rows_of for an incoming gradient, which may have any layout (an expanded scalar)."""
+    if not (t.dim() == 2 and t.stride(1) == 1):
+        t = t.contiguous()
+    return rows_of(t, what)
+
+
+def _same(what: str, x: torch.Tensor, t: Optional[torch.Tensor], name: str) -> None:
+    if t is None:
+        return
+    if t.device != x.device:
+        raise ValueError(f"{what}: {name} on {t.device}, x on {x.device}")
+    if t.dtype != x.dtype:
+        raise TypeError(f"{what}: {name} is {t.dtype}, x is {x.dtype}")
+    if t.shape != x.shape:
+        raise ValueError(f"{what}: {name} is {tuple(t.shape)}, x is {tuple(x.shape)}")
+
+
+def _drop_args(what: str, x: torch.Tensor, p: float, seed: Seed, site: int, row0: int,
+               negative_slope: float):
+    """(p, seed tensor or None, site, row0, slope, host seed), checked."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{what}: p must be between 0 and 1, got {p}")
+    if not 0 <= int(site) < 2 ** 32:
+        raise ValueError(f"{what}: site must be a 32-bit number, got {site}")
+    if int(row0) < 0:
+        raise ValueError(f"{what}: row0 must not be negative, got {row0}")
+    tensor = None
+    if isinstance(seed, torch.Tensor):
+        if seed.numel() != 1 or seed.dtype != torch.int64:
+            raise TypeError(f"{what}: a seed tensor holds one int64, got {seed.dtype} "
+                            f"{tuple(seed.shape)}")
+        if seed.device != x.device:
+            raise ValueError(f"{what}: seed on {seed.device}, x on {x.device}")
+        tensor, seed = seed, 0
+    return p, tensor, int(site), int(row0), float(negative_slope), int(seed) & (2 ** 64 - 1)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed_t, site, row0, slope, seed):
+        x2 = rows_of(x, "dropout")
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        rows, d = x2.shape
+        launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, ptr(x2),
+               x2.stride(0), ptr(y), d, p, seed, ptr(seed_t), site, row0, slope)
+        ctx.save_for_backward(x if slope != 1.0 else None, seed_t)
+        ctx.cfg = (p, site, row0, slope, seed)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, seed_t = ctx.saved_tensors
+        p, site, row0, slope, seed = ctx.cfg
+        dy2 = _rows_or_copy(dy, "dropout")
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        rows, d = dy2.shape
+        x2 = rows_of(x, "dropout") if x is not None else None
+        launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x2),
+               x2.stride(0) if x2 is not None else 0, ptr(dy2), dy2.stride(0), ptr(dx), d, p,
+               seed, ptr(seed_t), site, row0, slope)
+        return dx, None, None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed: Seed, *, site: int = 0, row0: int = 0,
+            negative_slope: float = 1.0) -> torch.Tensor:
+    """Dropout of LeakyReLU(x) (negative_slope 1: of x) with a mask that is never stored; see
+    the module's text for the mask, `seed`, `site` and `row0`. p = 1 drops everything, p = 0
+    nothing. p counts in steps of 1 / 65536, and the scale goes by the step used."""
+    rows_of(x, "dropout")
+    return _Dropout.apply(x, *_drop_args("dropout", x, p, seed, site, row0, negative_slope))
+
+
+class _NormBlock(torch.autograd.Function):
+    """(y, h) = (LN(h) w + b, h), h = residual + dropout(leaky(x)); h is None without `keep_h`
+    (layer_norm alone: h is x)."""
+
+    @staticmethod
+    def forward(ctx, what, keep_h, x, res, w, b, eps, p, seed_t, site, row0, slope, seed):
+        ctx.set_materialize_grads(False)
+        x2 = rows_of(x, what)
+        r2 = rows_of(res, what) if res is not None else None
+        rows, d = x2.shape
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = torch.empty_like(y) if keep_h else None
+        param = w if w is not None else b
+        wt = _lib.DTYPES[param.dtype if param is not None else x.dtype]
+        launch("gnnrec_layer_norm_forward", x.device, _lib.DTYPES[x.dtype], wt, rows, d, ptr(x2),
+               x2.stride(0), ptr(r2), r2.stride(0) if r2 is not None else 0, ptr(w), ptr(b), eps,
+               p, seed, ptr(seed_t), site, row0, slope, ptr(y), d, ptr(h), d)
+        ctx.save_for_backward(x, res, w, seed_t)
+        ctx.cfg = (what, wt, eps, p, site, row0, slope, seed, b is not None,
+                   b.dtype if b is not None else None)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        x, res, w, seed_t = ctx.saved_tensors
+        what, wt, eps, p, site, row0, slope, seed, has_b, b_dtype = ctx.cfg
+        need_x, need_r, need_w, need_b = ctx.needs_input_grad[2:6]
+        if dy is None and dh is None:
+            return (None,) * 13
+        x2 = rows_of(x, what)
+        r2 = rows_of(res, what) if res is not None else None
+        rows, d = x2.shape
+        if dy is None:      # only h was used: nothing passes through the norm
+            dy = torch.zeros_like(dh)
+        dy2 = _rows_or_copy(dy, what)
+        dh2 = _rows_or_copy(dh, what) if dh is not None else None
+        new = dict(dtype=x.dtype, device=x.device)
+        dx = torch.empty(x.shape, **new) if need_x else None
+        dres = torch.empty(x.shape, **new) if need_r else None
+        dw = torch.empty_like(w) if need_w else None
+        db = torch.empty(d, dtype=b_dtype, device=x.device) if need_b else None
+        work = None
+        if need_w or need_b:
+            work = torch.empty(_lib.lib().gnnrec_layer_norm_work_floats(rows, d),
+                               dtype=torch.float32, device=x.device)
+        launch("gnnrec_layer_norm_backward", x.device, _lib.DTYPES[x.dtype], wt, rows, d, ptr(x2),
+               x2.stride(0), ptr(r2), r2.stride(0) if r2 is not None else 0, ptr(w), eps, p, seed,
+               ptr(seed_t), site, row0, slope, ptr(dy2), dy2.stride(0), ptr(dh2),
+               dh2.stride(0) if dh2 is not None else 0, ptr(dx), d, ptr(dres), d, ptr(dw),
+               ptr(db), ptr(work))
+        return None, None, dx, dres, dw, db, None, None, None, None, None, None, None
+
+
+def _norm_args(what: str, x: torch.Tensor, weight, bias, eps: float) -> None:
+    rows_of(x, what)
+    d = x.shape[-1]
+    if d > MAX_NORM_WIDTH:
+        raise NotImplementedError(f"{what}: rows of {d} values, at most {MAX_NORM_WIDTH}")
+    if not eps >= 0.0:
+        raise ValueError(f"{what}: eps must not be negative, got {eps}")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise ValueError(f"{what}: {name} on {t.device}, x on {x.device}")
+        if t.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"{what}: {name} is {t.dtype}, expected {x.dtype} or float32")
+        if t.shape != (d,) or (d > 1 and t.stride(0) != 1):
+            raise ValueError(f"{what}: {name} must be a dense vector of {d} values")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"{what}: weight is {weight.dtype}, bias is {bias.dtype}")
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over x's last dimension (at most
+    MAX_NORM_WIDTH values; var divides by their number). weight and bias: x's dtype or float32,
+    either may be None. Gradients of x, weight and bias; the weight's and the bias's are summed
+    over all rows in fp32 in a fixed order."""
+    _norm_args("layer_norm", x, weight, bias, eps)
+    return _NormBlock.apply("layer_norm", False, x, None, weight, bias, float(eps), 0.0, None, 0,
+                            0, 1.0, 0)[0]
+
+
+def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
+                           weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                           p: float, seed: Seed, *, site: int = 0, row0: int = 0,
+                           negative_slope: float = 1.0, eps: float = 1e-5
+                           ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One layer's block in one pass: h = residual + dropout(LeakyReLU(x)) and y = LN(h) weight
+    + bias; returns (y, h). residual None: h = dropout(LeakyReLU(x)). The mask is dropout()'s for
+    the same p, seed, site and row0; the norm is layer_norm()'s, of the unrounded h."""
+    what = "dropout_add_layer_norm"
+    _norm_args(what, x, weight, bias, eps)
+    if residual is not None:
+        _same(what, x, residual, "residual")
+        rows_of(residual, what)
+    return _NormBlock.apply(what, True, x, residual, weight, bias, float(eps),
+                            *_drop_args(what, x, p, seed, site, row0, negative_slope))

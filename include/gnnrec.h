@@ -19,7 +19,8 @@
  *     offsets into col/val, row_ptr[0] need not be 0), `col[]` (int32, ascending within
  *     each row), `val[]` (fp32). Ascending columns are what makes the SpMM bit-exact with
  *     the reference's COO `torch.sparse.mm` (per-row sequential fmaf, col order).
- *   - Dense tables are fp32 row-major with an explicit leading dimension in ELEMENTS.
+ *   - Dense tables are fp32 row-major with an explicit leading dimension in ELEMENTS (the
+ *     row-wise entries at the end take a gnnrec_dtype; their rows may start at any element).
  */
 #ifndef GNNREC_H_
 #define GNNREC_H_
@@ -30,7 +31,7 @@
 extern "C" {
 #endif
 
-#define GNNREC_ABI_VERSION 11
+#define GNNREC_ABI_VERSION 12
 
 typedef struct ihipStream_t* gnnrec_stream_t;
 
@@ -40,6 +41,9 @@ enum gnnrec_status {
   GNNREC_EHIP = -2,         /* a HIP runtime call failed (launch error) */
   GNNREC_EUNSUPPORTED = -3  /* combination not implemented */
 };
+
+/* Element types of the row-wise entries (dropout, layer norm, 4-bit tables). */
+enum gnnrec_dtype { GNNREC_F32 = 0, GNNREC_BF16 = 1, GNNREC_F16 = 2 };
 
 /* Epilogue flags of gnnrec_spmm_csr_f32 (bit set). They fuse the LightGCN layer mean
  * `torch.stack(all_embeddings).mean(0)` (baselines/lightgcn.py:94-95) into the hop:
@@ -628,6 +632,72 @@ int gnnrec_adam_step_f32(float* param, const float* grad, float* exp_avg, float*
                          int64_t n, float step_size, double beta1, double beta2,
                          float bias_correction2_sqrt, float eps, float weight_decay,
                          const float* grad_scale, gnnrec_stream_t stream);
+
+/* ---- row-wise operators of the training path ---------------------------------------------
+ * Tables of `rows` rows of d values (dtype: gnnrec_dtype), leading dimensions in elements (0 is
+ * allowed for an input: one row for all). 32-bit arithmetic, one rounding at the store.
+ *
+ * Dropout with a LeakyReLU in front, as NGCF's layers end (baselines/ngcf.py:84-86: dropout of
+ * the activation; slope 1: no activation), from a counter-based generator instead of a stored
+ * mask. A value is dropped when its 16-bit draw is below round(p * 65536) (p in [0, 1]) and
+ * scaled by 65536 / (65536 - round(p * 65536)) otherwise. The draws are Philox4x32-10 with key =
+ * seed and counter = (column / 8, row0 + row, site), eight columns a block, so a value's fate
+ * depends on its place alone and the backward pass draws it again. seed_ptr, if not NULL, is a
+ * device int64 read instead of `seed` (a captured graph then replays with new masks). A dropped
+ * value is 0 whatever the input holds there. `site` tells the dropouts of one step apart.
+ *   forward : y  = keep ? act(x) * s : 0
+ *   backward: dx = keep ? dy * s * act'(x) : 0     (x may be NULL when slope == 1) */
+int gnnrec_dropout_forward(int32_t dtype, int64_t rows, int64_t d, const void* x, int64_t ldx,
+                           void* y, int64_t ldy, double p, uint64_t seed,
+                           const int64_t* seed_ptr, uint32_t site, int64_t row0, float slope,
+                           gnnrec_stream_t stream);
+int gnnrec_dropout_backward(int32_t dtype, int64_t rows, int64_t d, const void* x, int64_t ldx,
+                            const void* dy, int64_t lddy, void* dx, int64_t lddx, double p,
+                            uint64_t seed, const int64_t* seed_ptr, uint32_t site, int64_t row0,
+                            float slope, gnnrec_stream_t stream);
+
+/* Layer norm of h = res + dropout(act(x)) (res may be NULL; p = 0 and slope = 1: of res + x),
+ * 1 <= d <= 16384:
+ *   y = (h - mean(h)) / sqrt(var(h) + eps) * w + b   (w, b of dtype wdtype: the table's or
+ * GNNREC_F32; either may be NULL: 1 and 0). h, if not NULL, receives the sum (rounded; the
+ * statistics are those of the unrounded sum).
+ * Backward, from the same inputs (h and the statistics are formed again): dy, and dh (may be
+ * NULL) the gradient that reaches h by itself. dx, dres, dw, db may each be NULL. dw / db are
+ * sums over all rows in a fixed order; they need `work`, gnnrec_layer_norm_work_floats(rows, d)
+ * floats of scratch that no call running at the same time uses. */
+int gnnrec_layer_norm_forward(int32_t dtype, int32_t wdtype, int64_t rows, int64_t d,
+                              const void* x, int64_t ldx, const void* res, int64_t ldr,
+                              const void* w, const void* b, float eps, double p, uint64_t seed,
+                              const int64_t* seed_ptr, uint32_t site, int64_t row0, float slope,
+                              void* y, int64_t ldy, void* h, int64_t ldh,
+                              gnnrec_stream_t stream);
+int64_t gnnrec_layer_norm_work_floats(int64_t rows, int64_t d);
+int gnnrec_layer_norm_backward(int32_t dtype, int32_t wdtype, int64_t rows, int64_t d,
+                               const void* x, int64_t ldx, const void* res, int64_t ldr,
+                               const void* w, float eps, double p, uint64_t seed,
+                               const int64_t* seed_ptr, uint32_t site, int64_t row0, float slope,
+                               const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                               void* dx, int64_t lddx, void* dres, int64_t lddr, void* dw,
+                               void* db, float* work, gnnrec_stream_t stream);
+
+/* ---- item tables in 4 bits ---------------------------------------------------------------
+ * n rows of k values as E2M1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte
+ * with the even column in the low half, each row padded to G = ceil(k / 32) groups of 16 bytes
+ * (what the padding holds does not matter), and one bfloat16 scale per group: codes [n, 16 G]
+ * bytes, 16-B aligned; scale [n, G]. value = e2m1(code) * scale.
+ * quantize: scale = bf16(largest magnitude of the group / 6), code = nearest, ties to the even
+ * code; a group with an infinity or a NaN gets a NaN scale. */
+int gnnrec_quantize_q4(int32_t dtype, int64_t n, int64_t k, const void* w, int64_t ldw,
+                       void* codes, void* scale, gnnrec_stream_t stream);
+int gnnrec_dequantize_q4(int64_t n, int64_t k, const void* codes, const void* scale, float* out,
+                         int64_t ldo, gnnrec_stream_t stream);
+
+/* out[i, r] = sum_c x[i, c] * value[r, c]: scores of m <= 65535 users' rows (x: [m, k] of dtype)
+ * against all n items of a 4-bit table, as user_emb @ item_emb.T (evaluator.py:96) does with
+ * full-width items. The products are exact and summed in fp32; out is [m, n] of out_dtype. */
+int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, const void* x, int64_t ldx,
+                     int64_t n, int64_t k, const void* codes, const void* scale, void* out,
+                     int64_t ldo, gnnrec_stream_t stream);
 
 #ifdef __cplusplus
 }
