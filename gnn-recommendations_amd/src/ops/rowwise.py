@@ -36,14 +36,25 @@ MAX_NORM_WIDTH = 16384    # csrc/layer_norm.hip kNormMaxD
 Seed = Union[int, torch.Tensor]
 
 
+_ENTRIES: dict = {}
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream, less the objects
+
+
 def launch(name: str, device: torch.device, *args) -> None:
-    """Call a C entry on `device`'s current stream, whatever device is current."""
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, _lib.stream_of(device)), name)
+    """Call a C entry on `device`'s current stream, whatever device is current. The calls of a
+    small table cost the host more than the GPU, so nothing is looked up twice here."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(_lib.lib(), name)
+    i = device.index
+    if _current_device() == i:
+        rc = fn(*args, _raw_stream(i))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _lib.stream_of(device)), name)
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        check(rc, name)
 
 
 def rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -62,11 +73,16 @@ def rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
                      "tensor")
 
 
-def _rows_or_copy(t: torch.Tensor, what: str) -> torch.Tensor:
-    """rows_of for an incoming gradient, which may have any layout (an expanded scalar)."""
-    if not (t.dim() == 2 and t.stride(1) == 1):
-        t = t.contiguous()
-    return rows_of(t, what)
+def _dense_rows(t: Optional[torch.Tensor]):
+    """(tensor, row stride) in a backward pass, of an incoming gradient (which may have any
+    layout: an expanded scalar) or of a saved tensor (which a saved-tensor hook may have laid
+    out anew): a 2-D row-major one as it is, another as a contiguous tensor."""
+    if t is None:
+        return None, 0
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0)
+    t = t.contiguous()
+    return t, t.shape[-1]
 
 
 def _same(what: str, x: torch.Tensor, t: Optional[torch.Tensor], name: str) -> None:
@@ -101,31 +117,37 @@ def _drop_args(what: str, x: torch.Tensor, p: float, seed: Seed, site: int, row0
     return p, tensor, int(site), int(row0), float(negative_slope), int(seed) & (2 ** 64 - 1)
 
 
+def _once(backward):
+    """once_differentiable(backward), without its cost where no second derivative is asked for."""
+    guarded = once_differentiable(backward)
+
+    def wrapped(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return staticmethod(wrapped)
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, p, seed_t, site, row0, slope, seed):
-        x2 = rows_of(x, "dropout")
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        rows, d = x2.shape
-        launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, ptr(x2),
-               x2.stride(0), ptr(y), d, p, seed, ptr(seed_t), site, row0, slope)
+    def forward(ctx, x, ldx, rows, p, seed_t, site, row0, slope, seed):
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        d = x.shape[-1]
+        launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, x.data_ptr(),
+               ldx, y.data_ptr(), d, p, seed, ptr(seed_t), site, row0, slope)
         ctx.save_for_backward(x if slope != 1.0 else None, seed_t)
-        ctx.cfg = (p, site, row0, slope, seed)
+        ctx.cfg = (rows, p, site, row0, slope, seed)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, seed_t = ctx.saved_tensors
-        p, site, row0, slope, seed = ctx.cfg
-        dy2 = _rows_or_copy(dy, "dropout")
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-        rows, d = dy2.shape
-        x2 = rows_of(x, "dropout") if x is not None else None
-        launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x2),
-               x2.stride(0) if x2 is not None else 0, ptr(dy2), dy2.stride(0), ptr(dx), d, p,
-               seed, ptr(seed_t), site, row0, slope)
-        return dx, None, None, None, None, None, None
+        rows, p, site, row0, slope, seed = ctx.cfg
+        x, ldx = _dense_rows(x)
+        dy, lddy = _dense_rows(dy)
+        dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+        d = dy.shape[-1]
+        launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x), ldx,
+               dy.data_ptr(), lddy, dx.data_ptr(), d, p, seed, ptr(seed_t), site, row0, slope)
+        return dx, None, None, None, None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: Seed, *, site: int = 0, row0: int = 0,
@@ -133,8 +155,8 @@ def dropout(x: torch.Tensor, p: float, seed: Seed, *, site: int = 0, row0: int =
     """Dropout of LeakyReLU(x) (negative_slope 1: of x) with a mask that is never stored; see
     the module's text for the mask, `seed`, `site` and `row0`. p = 1 drops everything, p = 0
     nothing. p counts in steps of 1 / 65536, and the scale goes by the step used."""
-    rows_of(x, "dropout")
-    return _Dropout.apply(x, *_drop_args("dropout", x, p, seed, site, row0, negative_slope))
+    x2 = rows_of(x, "dropout")
+    return _Dropout.apply(x, x2.stride(0), x2.shape[0], *_drop_args("dropout", x, p, seed, site, row0, negative_slope))
 
 
 class _NormBlock(torch.autograd.Function):
@@ -142,58 +164,55 @@ class _NormBlock(torch.autograd.Function):
     (layer_norm alone: h is x)."""
 
     @staticmethod
-    def forward(ctx, what, keep_h, x, res, w, b, eps, p, seed_t, site, row0, slope, seed):
+    def forward(ctx, keep_h, x, ldx, rows, res, ldr, w, b, eps, p, seed_t, site, row0, slope,
+                seed):
         ctx.set_materialize_grads(False)
-        x2 = rows_of(x, what)
-        r2 = rows_of(res, what) if res is not None else None
-        rows, d = x2.shape
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
         h = torch.empty_like(y) if keep_h else None
-        param = w if w is not None else b
-        wt = _lib.DTYPES[param.dtype if param is not None else x.dtype]
-        launch("gnnrec_layer_norm_forward", x.device, _lib.DTYPES[x.dtype], wt, rows, d, ptr(x2),
-               x2.stride(0), ptr(r2), r2.stride(0) if r2 is not None else 0, ptr(w), ptr(b), eps,
-               p, seed, ptr(seed_t), site, row0, slope, ptr(y), d, ptr(h), d)
+        d = x.shape[-1]
+        t = _lib.DTYPES[x.dtype]
+        wt = t if w is None and b is None else _lib.DTYPES[(b if w is None else w).dtype]
+        launch("gnnrec_layer_norm_forward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res),
+               ldr, ptr(w), ptr(b), eps, p, seed, ptr(seed_t), site, row0, slope, y.data_ptr(), d,
+               ptr(h), d)
         ctx.save_for_backward(x, res, w, seed_t)
-        ctx.cfg = (what, wt, eps, p, site, row0, slope, seed, b is not None,
+        ctx.cfg = (rows, t, wt, eps, p, site, row0, slope, seed,
                    b.dtype if b is not None else None)
         return y, h
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dh):
         x, res, w, seed_t = ctx.saved_tensors
-        what, wt, eps, p, site, row0, slope, seed, has_b, b_dtype = ctx.cfg
-        need_x, need_r, need_w, need_b = ctx.needs_input_grad[2:6]
+        rows, t, wt, eps, p, site, row0, slope, seed, b_dtype = ctx.cfg
+        need = ctx.needs_input_grad
+        need_w, need_b = need[6], need[7]
         if dy is None and dh is None:
-            return (None,) * 13
-        x2 = rows_of(x, what)
-        r2 = rows_of(res, what) if res is not None else None
-        rows, d = x2.shape
+            return (None,) * 15
         if dy is None:      # only h was used: nothing passes through the norm
             dy = torch.zeros_like(dh)
-        dy2 = _rows_or_copy(dy, what)
-        dh2 = _rows_or_copy(dh, what) if dh is not None else None
-        new = dict(dtype=x.dtype, device=x.device)
-        dx = torch.empty(x.shape, **new) if need_x else None
-        dres = torch.empty(x.shape, **new) if need_r else None
+        x, ldx = _dense_rows(x)
+        res, ldr = _dense_rows(res)
+        dy, lddy = _dense_rows(dy)
+        dh, lddh = _dense_rows(dh)
+        d = x.shape[-1]
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[1] else None
+        dres = torch.empty_like(x, memory_format=torch.contiguous_format) if need[4] else None
         dw = torch.empty_like(w) if need_w else None
-        db = torch.empty(d, dtype=b_dtype, device=x.device) if need_b else None
+        db = x.new_empty(d, dtype=b_dtype) if need_b else None
         work = None
         if need_w or need_b:
-            work = torch.empty(_lib.lib().gnnrec_layer_norm_work_floats(rows, d),
-                               dtype=torch.float32, device=x.device)
-        launch("gnnrec_layer_norm_backward", x.device, _lib.DTYPES[x.dtype], wt, rows, d, ptr(x2),
-               x2.stride(0), ptr(r2), r2.stride(0) if r2 is not None else 0, ptr(w), eps, p, seed,
-               ptr(seed_t), site, row0, slope, ptr(dy2), dy2.stride(0), ptr(dh2),
-               dh2.stride(0) if dh2 is not None else 0, ptr(dx), d, ptr(dres), d, ptr(dw),
-               ptr(db), ptr(work))
-        return None, None, dx, dres, dw, db, None, None, None, None, None, None, None
+            work = x.new_empty(_lib.lib().gnnrec_layer_norm_work_floats(rows, d),
+                               dtype=torch.float32)
+        launch("gnnrec_layer_norm_backward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res),
+               ldr, ptr(w), eps, p, seed, ptr(seed_t), site, row0, slope, dy.data_ptr(), lddy,
+               ptr(dh), lddh, ptr(dx), d, ptr(dres), d, ptr(dw), ptr(db), ptr(work))
+        return (None, dx, None, None, dres, None, dw, db) + (None,) * 7
 
 
-def _norm_args(what: str, x: torch.Tensor, weight, bias, eps: float) -> None:
-    rows_of(x, what)
-    d = x.shape[-1]
+def _norm_args(what: str, x: torch.Tensor, weight, bias, eps: float):
+    """(row stride, rows) of x, everything checked."""
+    x2 = rows_of(x, what)
+    rows, d = x2.shape
     if d > MAX_NORM_WIDTH:
         raise NotImplementedError(f"{what}: rows of {d} values, at most {MAX_NORM_WIDTH}")
     if not eps >= 0.0:
@@ -209,6 +228,7 @@ def _norm_args(what: str, x: torch.Tensor, weight, bias, eps: float) -> None:
             raise ValueError(f"{what}: {name} must be a dense vector of {d} values")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"{what}: weight is {weight.dtype}, bias is {bias.dtype}")
+    return x2.stride(0), rows
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -217,8 +237,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     MAX_NORM_WIDTH values; var divides by their number). weight and bias: x's dtype or float32,
     either may be None. Gradients of x, weight and bias; the weight's and the bias's are summed
     over all rows in fp32 in a fixed order."""
-    _norm_args("layer_norm", x, weight, bias, eps)
-    return _NormBlock.apply("layer_norm", False, x, None, weight, bias, float(eps), 0.0, None, 0,
+    ldx, rows = _norm_args("layer_norm", x, weight, bias, eps)
+    return _NormBlock.apply(False, x, ldx, rows, None, 0, weight, bias, float(eps), 0.0, None, 0,
                             0, 1.0, 0)[0]
 
 
@@ -231,9 +251,10 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     + bias; returns (y, h). residual None: h = dropout(LeakyReLU(x)). The mask is dropout()'s for
     the same p, seed, site and row0; the norm is layer_norm()'s, of the unrounded h."""
     what = "dropout_add_layer_norm"
-    _norm_args(what, x, weight, bias, eps)
+    ldx, rows = _norm_args(what, x, weight, bias, eps)
+    ldr = 0
     if residual is not None:
         _same(what, x, residual, "residual")
-        rows_of(residual, what)
-    return _NormBlock.apply(what, True, x, residual, weight, bias, float(eps),
+        ldr = rows_of(residual, what).stride(0)
+    return _NormBlock.apply(True, x, ldx, rows, residual, ldr, weight, bias, float(eps),
                             *_drop_args(what, x, p, seed, site, row0, negative_slope))

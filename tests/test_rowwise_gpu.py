@@ -281,6 +281,27 @@ def test_views_and_ranks(cuda):
     assert torch.equal(dr, torch.full_like(dr, 60.0))
 
 
+def test_saved_tensor_hooks(cuda):
+    """A hook may give a saved view back with another layout (as one kept on the host is)."""
+    wide, wide2 = _randn(40, 200), _randn(40, 200, seed=1)
+    dy = _randn(40, 64, seed=2)
+
+    def grads():
+        x, r = (t[:, 3:67].detach().requires_grad_() for t in (wide, wide2))
+        y, h = ops.dropout_add_layer_norm(x, r, None, None, 0.2, 5, negative_slope=0.2)
+        z = ops.dropout(x, 0.2, 5, negative_slope=0.2)
+        return torch.autograd.grad((y, h, z), (x, r), (dy, dy, dy))
+
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone().t().contiguous().t()
+                                                  if t.dim() == 2 else t, lambda t: t):
+        other = grads()
+    for a, b, c in zip(want, got, other):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_no_rows(cuda):
     x = torch.empty(0, 64, device="cuda", requires_grad=True)
     w = torch.ones(64, device="cuda", requires_grad=True)
