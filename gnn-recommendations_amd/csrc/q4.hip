@@ -191,126 +191,119 @@ __device__ __forceinline__ void store_out(void* out, int32_t dtype, int64_t i, f
 }
 
 struct Q4Args {
-  int64_t m, ldx, n, k, ng, ldo;
+  int64_t m, n, k, ng, ldo;
   const uint32_t* codes;
   const bf16_t* scale;
   void* out;
   int32_t out_dtype;
 };
 
-// FEW: at most four users a tile. WK waves share 64 items and split the groups; WK == 1: every
-// wave takes items of its own. HELD > 0: rows of at most 4 HELD groups, whose users' fragments
-// stay in registers over all the wave's items.
-template <class T, bool FEW, int WK, int HELD>
-__global__ __launch_bounds__(WK > 4 ? WK * 64 : 256) void q4_matmul_kernel(
-    const T* __restrict__ x, Q4Args p) {
-  constexpr int kA = FEW ? 1 : Parts<T>::n;
-  constexpr int kWaves = WK > 4 ? WK : 4;
-  __shared__ f32x4 join[WK > 1 ? (WK - 1) * 4 * 64 : 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int r = lane & 15, q = lane >> 4;
-  const int64_t user0 = (int64_t)blockIdx.y * (FEW ? 4 : 16);
-  const int64_t user = user0 + (FEW ? (r & 3) : r);
-  const int part = FEW ? r >> 2 : 0;
-  const bool valid = user < p.m && part < Parts<T>::n;
-  const T* xrow = x + (user < p.m ? user : 0) * p.ldx;
-  const int64_t blocks4 = (p.ng + 3) >> 2;
-
-  bf16x8 held[HELD ? HELD * 4 : 1][kA];
-  if (HELD) {
+// acc[t] += the products of R groups from g0 on (R == 4: as many of four as the row has) of NT
+// tiles of 16 items. Rows are given as an offset from `base`, clamped to the table's last row (a
+// clamped row's results are not stored).
+//
+// Loads: with four groups, lane (q, r) takes 16 bytes, group g0 + q of row r of a tile; of rows
+// with only two (one) groups left, a load covers two (four) tiles, so that no lane idles and the
+// wave reads one contiguous piece. Either way word j of load i after the transposition holds
+// eight codes of one (tile, group) in every lane row. Scales: lane l takes those of row l of the
+// 64, and two swaps spread a tile's to all lane rows.
+template <int NT, int R, int KA, class A>
+__device__ __forceinline__ void groups(const Q4Args& p, int64_t base, int64_t g0, A&& users,
+                                       f32x4 (&acc)[NT]) {
+  static_assert(NT == 4 || (NT == 1 && R == 4), "a single tile always takes four groups");
+  constexpr int kLoads = NT == 4 ? R : 1;  // four tiles x R groups, four pieces of 16 B a load
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int last = (int)(p.n - 1 - base < 63 ? p.n - 1 - base : 63);
+  const uint32_t* codes = p.codes + (base * p.ng + g0) * 4;
+  const uint16_t* scale = reinterpret_cast<const uint16_t*>(p.scale) + base * p.ng + g0;
+  const int here = p.ng - g0 < 4 ? (int)(p.ng - g0) : 4;  // groups left
+  u32x4 w[kLoads];
 #pragma unroll
-    for (int g = 0; g < HELD * 4; ++g)
-      load_users<T, FEW>(xrow, valid, part, (int64_t)g * kGroup + q * 8, p.k, held[g]);
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = (R == 4 ? i * 16 : R == 2 ? i * 32 + (q >> 1) * 16 : q * 16) + r;
+    const int g = R == 4 ? q : R == 2 ? (q & 1) : 0;
+    w[i] = u32x4{0, 0, 0, 0};
+    if (R < 4 || g < here)
+      w[i] = *reinterpret_cast<const u32x4*>(
+          codes + ((int64_t)(row < last ? row : last) * p.ng + g) * 4);
   }
-  const int64_t tasks = (p.n + 63) >> 6;
-  const int64_t first = WK == 1 ? (int64_t)blockIdx.x * kWaves + wave : blockIdx.x;
-  const int64_t step = WK == 1 ? (int64_t)gridDim.x * kWaves : gridDim.x;
-  for (int64_t task = first; task < tasks; task += step) {
-    const int64_t base = task * 64;
-    int64_t row[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int64_t i = base + t * 16 + r;
-      row[t] = i < p.n ? i : p.n - 1;
-    }
-    f32x4 acc[4] = {};
-    auto step4 = [&](int64_t b, const bf16x8(*a)[kA]) {
-      const int64_t g0 = b * 4;
-      u32x4 w[4];
-      uint32_t sc[4][4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        w[t] = u32x4{0, 0, 0, 0};
-        if (g0 + q < p.ng)
-          w[t] = *reinterpret_cast<const u32x4*>(p.codes + (row[t] * p.ng + g0 + q) * 4);
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          sc[t][g] = g0 + g < p.ng
-                         ? (uint32_t)reinterpret_cast<const uint16_t*>(p.scale)[row[t] * p.ng + g0 + g]
-                         : 0;
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) transpose4(w[t]);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (g0 + g >= p.ng) break;
-        bf16x8 now[kA];
-        if (HELD) {
-#pragma unroll
-          for (int i = 0; i < kA; ++i) now[i] = a[g][i];
-        } else {
-          load_users<T, FEW>(xrow, valid, part, (g0 + g) * kGroup + q * 8, p.k, now);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const bf16x8 bf = codes_to_bf16(w[t][g]);
-          f32x4 d = {};
-#pragma unroll
-          for (int i = kA - 1; i >= 0; --i)
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(now[i], bf, d, 0, 0, 0);
-          const float s = __uint_as_float(sc[t][g] << 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(s, d[i], acc[t][i]);
-        }
-      }
-    };
-    if (HELD) {
-#pragma unroll
-      for (int b = 0; b < HELD; ++b) step4(b, held + b * 4);
+  // s[h]: scales of groups g0 + 2 h and g0 + 2 h + 1
+  uint32_t s[2] = {0, 0};
+  {
+    const int row = NT == 4 ? lane : r;
+    const uint16_t* at = scale + (int64_t)(row < last ? row : last) * p.ng;
+    struct __attribute__((packed)) Two { uint32_t v[2]; };
+    struct __attribute__((packed)) One { uint32_t v; };
+    if (R == 1) {
+      s[0] = at[0];
+    } else if (R == 2) {
+      s[0] = reinterpret_cast<const One*>(at)->v;
+    } else if (here == 4) {
+      const Two v = *reinterpret_cast<const Two*>(at);
+      s[0] = v.v[0], s[1] = v.v[1];
     } else {
-      const int64_t b0 = WK > 1 ? blocks4 * wave / WK : 0;
-      const int64_t b1 = WK > 1 ? blocks4 * (wave + 1) / WK : blocks4;
-      for (int64_t b = b0; b < b1; ++b) step4(b, held);
+      s[0] = at[0];
+      if (here > 1) s[0] |= (uint32_t)at[1] << 16;
+      if (here > 2) s[1] = at[2];
     }
-    if (WK > 1) {
-      if (wave > 0) {
+  }
+  uint32_t st[2][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) join[((wave - 1) * 4 + t) * 64 + lane] = acc[t];
-      }
-      __syncthreads();
-      if (wave == 0) {
-        for (int v = 0; v < WK - 1; ++v)
-#pragma unroll
-          for (int t = 0; t < 4; ++t) acc[t] += join[(v * 4 + t) * 64 + lane];
-      }
-      __syncthreads();
-      if (wave > 0) continue;
+  for (int h = 0; h < (R == 4 ? 2 : 1); ++h) {
+    if (NT == 1) {
+      st[h][0] = s[h];
+    } else {
+      uint32_t a = s[h], b = s[h];
+      swap16(a, b);  // rows (0 0 2 2) and (1 1 3 3)
+      uint32_t c = a, d = b;
+      swap32(a, c);
+      swap32(b, d);
+      st[h][0] = a, st[h][1] = b, st[h][2] = c, st[h][3] = d;
     }
-    // lane (q, r) holds users 4 q + i (or part q of user i) of items 16 t + r; with t and q
-    // exchanged, a register is one user's 64 neighbouring items
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) transpose4(w[i]);
+#pragma unroll
+  for (int g = 0; g < R; ++g) {
+    if (R == 4 && g >= here) break;
+    const auto& a = users(g);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint32_t word = R == 4 ? w[t][g] : R == 2 ? w[t >> 1][(t & 1) * 2 + g] : w[0][t];
+      const bf16x8 bf = codes_to_bf16(word);
+      f32x4 d = {};
+#pragma unroll
+      for (int i = KA - 1; i >= 0; --i)
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], bf, d, 0, 0, 0);
+      const uint32_t sw = st[g >> 1][t];
+      const float sc = __uint_as_float(g & 1 ? sw & 0xffff0000u : sw << 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(sc, d[i], acc[t][i]);
+    }
+  }
+}
+
+// The results of NT tiles. Lane (q, r) holds users 4 q + i of item r of a tile, or part q of user
+// i; a transposition gives a register 64 neighbouring items of one user (NT == 4), or the parts
+// of user q (FEW, NT == 1).
+template <bool FEW, int NT, int PARTS>
+__device__ __forceinline__ void store_tiles(const Q4Args& p, int64_t base, int64_t user0,
+                                            const f32x4 (&acc)[NT]) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  if (NT == 4) {
+    const int64_t item = base + lane;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (user0 + i >= p.m) break;
       u32x4 v;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) v[t] = __float_as_uint(acc[t][i]);
+      for (int t = 0; t < 4; ++t) v[t] = __float_as_uint(acc[t % NT][i]);
       transpose4(v);
-      const int64_t item = base + lane;
       if (FEW) {
         float s = __uint_as_float(v[0]);
 #pragma unroll
-        for (int j = 1; j < Parts<T>::n; ++j) s += __uint_as_float(v[j]);
-        if (user0 + i < p.m && item < p.n)
-          store_out(p.out, p.out_dtype, (user0 + i) * p.ldo + item, s);
+        for (int j = 1; j < PARTS; ++j) s += __uint_as_float(v[j]);
+        if (item < p.n) store_out(p.out, p.out_dtype, (user0 + i) * p.ldo + item, s);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -320,26 +313,195 @@ __global__ __launch_bounds__(WK > 4 ? WK * 64 : 256) void q4_matmul_kernel(
         }
       }
     }
+  } else {
+    const int64_t item = base + r;
+    if (FEW) {
+      u32x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(acc[0][i]);
+      transpose4(v);
+      float s = __uint_as_float(v[0]);
+#pragma unroll
+      for (int j = 1; j < PARTS; ++j) s += __uint_as_float(v[j]);
+      if (user0 + q < p.m && item < p.n)
+        store_out(p.out, p.out_dtype, (user0 + q) * p.ldo + item, s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t u = user0 + 4 * q + i;
+        if (u < p.m && item < p.n) store_out(p.out, p.out_dtype, u * p.ldo + item, acc[0][i]);
+      }
+    }
   }
 }
 
+// Short rows (at most 8 groups, 256 columns): the users' fragments stay in registers over all the
+// items of a wave. FEW: at most four users a tile, the parts in the instruction's idle rows. HELD
+// steps of four groups, the last of R.
+template <class T, bool FEW, int NT, int HELD, int R>
+__global__ __launch_bounds__(kQ4Block) void q4_short_kernel(const T* __restrict__ x, int64_t ldx,
+                                                            Q4Args p) {
+  constexpr int kA = FEW ? 1 : Parts<T>::n;
+  constexpr int kHeld = (HELD - 1) * 4 + R;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const int64_t user0 = (int64_t)blockIdx.y * (FEW ? 4 : 16);
+  const int64_t user = user0 + (FEW ? (r & 3) : r);
+  const int part = FEW ? r >> 2 : 0;
+  const bool valid = user < p.m && part < Parts<T>::n;
+  bf16x8 held[kHeld][kA];
+#pragma unroll
+  for (int g = 0; g < kHeld; ++g)
+    load_users<T, FEW>(x + (valid ? user : 0) * ldx, valid, part, (int64_t)g * kGroup + q * 8, p.k,
+                       held[g]);
+  const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16);
+  for (int64_t task = (int64_t)blockIdx.x * 4 + wave; task < tasks; task += (int64_t)gridDim.x * 4) {
+    const int64_t base = task * NT * 16;
+    f32x4 acc[NT] = {};
+    if (HELD == 2)
+      groups<NT, 4, kA>(p, base, 0, [&](int g) -> auto& { return held[g % kHeld]; }, acc);
+    groups<NT, R, kA>(p, base, (HELD - 1) * 4,
+                      [&](int g) -> auto& { return held[(HELD - 1) * 4 + g]; }, acc);
+    store_tiles<FEW, NT, Parts<T>::n>(p, base, user0, acc);
+  }
+}
+
+// Long rows: the users come as bf16 parts (plane i at x + i * plane, rows ldx apart), from the
+// table itself or from split_users_kernel. WK waves share a tile set and split its groups; their
+// sums are joined through LDS in the waves' order.
+template <int PARTS, bool FEW, int NT, int WK>
+__global__ __launch_bounds__(WK > 4 ? WK * 64 : 256) void q4_long_kernel(
+    const bf16_t* __restrict__ x, int64_t ldx, int64_t plane, Q4Args p) {
+  constexpr int kA = FEW ? 1 : PARTS;
+  __shared__ f32x4 join[WK > 1 ? (WK - 1) * NT * 64 : 1];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const int64_t user0 = (int64_t)blockIdx.y * (FEW ? 4 : 16);
+  const int64_t user = user0 + (FEW ? (r & 3) : r);
+  const int part = FEW ? r >> 2 : 0;
+  const bool valid = user < p.m && part < PARTS;
+  const bf16_t* xrow = x + (valid ? part * plane + user * ldx : 0);
+  const int64_t blocks4 = (p.ng + 3) >> 2;
+  const int64_t b0 = WK > 1 ? blocks4 * wave / WK : 0;
+  const int64_t b1 = WK > 1 ? blocks4 * (wave + 1) / WK : blocks4;
+  const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16);
+  const int64_t first = WK > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int64_t step = WK > 1 ? gridDim.x : (int64_t)gridDim.x * 4;
+  for (int64_t task = first; task < tasks; task += step) {
+    const int64_t base = task * NT * 16;
+    f32x4 acc[NT] = {};
+#pragma unroll 2
+    for (int64_t b = b0; b < b1; ++b) {
+      bf16x8 a[4][kA];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int64_t c = (b * 4 + g) * kGroup + q * 8;
+#pragma unroll
+        for (int i = 0; i < kA; ++i) {
+          a[g][i] = bf16x8{};
+          if (valid && c + 8 <= p.k) {
+            a[g][i] = __builtin_bit_cast(
+                bf16x8, *reinterpret_cast<const Eight<bf16_t>*>(xrow + i * plane + c));
+          } else if (valid && c < p.k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < p.k) a[g][i][e] = xrow[i * plane + c + e];
+          }
+        }
+      }
+      groups<NT, 4, kA>(p, base, b * 4, [&](int g) -> auto& { return a[g]; }, acc);
+    }
+    if (WK > 1) {
+      if (wave > 0) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) join[((wave - 1) * NT + t) * 64 + lane] = acc[t];
+      }
+      __syncthreads();
+      if (wave == 0) {
+        for (int v = 0; v < WK - 1; ++v)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[t] += join[(v * NT + t) * 64 + lane];
+      }
+      __syncthreads();  // the sums have been read before the next task's are written
+      if (wave > 0) continue;
+    }
+    store_tiles<FEW, NT, PARTS>(p, base, user0, acc);
+  }
+}
+
+// x [m, k] as bf16 parts: plane i, rows of kp = 32 ng values, zeros behind k.
+template <class T>
+__global__ __launch_bounds__(kQ4Block) void split_users_kernel(const T* __restrict__ x,
+                                                               int64_t ldx, int64_t m, int64_t k,
+                                                               int64_t kp,
+                                                               bf16_t* __restrict__ parts) {
+  constexpr int kP = Parts<T>::n;
+  const int64_t i = (int64_t)blockIdx.x * kQ4Block + threadIdx.x;
+  const int64_t per = kp / 8, row = i / per, c = (i - row * per) * 8;
+  if (row >= m) return;
+  float v[8];
+  load8(x + row * ldx + c, k - c, v);
+#pragma unroll
+  for (int j = 0; j < kP; ++j) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t lo = cut(v[2 * e]), hi = cut(v[2 * e + 1]);
+      w[e] = (lo >> 16) | hi;
+    }
+    *reinterpret_cast<u32x4*>(parts + (j * m + row) * kp + c) = w;
+  }
+}
+
+constexpr int64_t kShortGroups = 8;
+
 template <class T, bool FEW>
-static int run_matmul(const T* x, const Q4Args& p, hipStream_t stream) {
-  const int64_t tasks = ceil_div(p.n, 64);
-  const unsigned tiles = (unsigned)ceil_div(p.m, FEW ? 4 : 16);
-  auto go = [&](auto wk, auto held) {
-    constexpr int kWaves = wk.value > 4 ? wk.value : 4;
-    const int64_t want = wk.value == 1 ? ceil_div(tasks, 4) : tasks;
-    const unsigned grid = (unsigned)(want < 2048 ? want : 2048);
-    hipLaunchKernelGGL((q4_matmul_kernel<T, FEW, wk.value, held.value>), dim3(grid, tiles),
-                       dim3(kWaves * 64), 0, stream, x, p);
+static int run_short(const T* x, int64_t ldx, const Q4Args& p, hipStream_t stream) {
+  auto go = [&](auto nt, auto held, auto rem) {
+    const int64_t want = ceil_div(ceil_div(p.n, nt.value * 16), 4);
+    hipLaunchKernelGGL((q4_short_kernel<T, FEW, nt.value, held.value, rem.value>),
+                       dim3((unsigned)(want < 2048 ? want : 2048),
+                            (unsigned)ceil_div(p.m, FEW ? 4 : 16)),
+                       dim3(kQ4Block), 0, stream, x, ldx, p);
     return check_launch("q4_matmul");
   };
   using std::integral_constant;
-  if (p.ng <= 4) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  if (p.ng <= 8) return go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-  if (p.ng < 64) return go(integral_constant<int, 4>{}, integral_constant<int, 0>{});
-  return go(integral_constant<int, 16>{}, integral_constant<int, 0>{});
+  const integral_constant<int, 1> i1{};
+  const integral_constant<int, 2> i2{};
+  const integral_constant<int, 4> i4{};
+  if (p.n < 64 * 1024) {  // one tile a wave: four times the waves
+    if (p.ng <= 4) return go(i1, i1, i4);
+    return go(i1, i2, i4);
+  }
+  switch (p.ng) {
+    case 1: return go(i4, i1, i1);
+    case 2: return go(i4, i1, i2);
+    case 3: case 4: return go(i4, i1, i4);
+    case 5: return go(i4, i2, i1);
+    case 6: return go(i4, i2, i2);
+    default: return go(i4, i2, i4);
+  }
+}
+
+template <int PARTS, bool FEW>
+static int run_long(const bf16_t* x, int64_t ldx, int64_t plane, const Q4Args& p,
+                    hipStream_t stream) {
+  auto go = [&](auto nt, auto wk) {
+    const int64_t tasks = ceil_div(p.n, nt.value * 16);
+    const int64_t want = wk.value == 1 ? ceil_div(tasks, 4) : tasks;
+    hipLaunchKernelGGL((q4_long_kernel<PARTS, FEW, nt.value, wk.value>),
+                       dim3((unsigned)(want < 4096 ? want : 4096),
+                            (unsigned)ceil_div(p.m, FEW ? 4 : 16)),
+                       dim3(wk.value > 4 ? wk.value * 64 : 256), 0, stream, x, ldx, plane, p);
+    return check_launch("q4_matmul");
+  };
+  using std::integral_constant;
+  const integral_constant<int, 1> i1{};
+  const integral_constant<int, 4> i4{};
+  const integral_constant<int, 8> i8{};
+  if (p.n >= 64 * 4096) return go(i4, i1);
+  if (p.n >= 64 * 512) return go(i4, i4);
+  return p.ng >= 32 ? go(i1, i8) : go(i1, i4);
 }
 
 static int check_table(const char* what, int64_t n, int64_t k, const void* codes,
@@ -385,9 +547,15 @@ extern "C" int gnnrec_dequantize_q4(int64_t n, int64_t k, const void* codes, con
   return check_launch("dequantize_q4");
 }
 
+extern "C" int64_t gnnrec_q4_matmul_work_bytes(int32_t dtype, int64_t m, int64_t k) {
+  const int64_t ng = ceil_div(k, kGroup);
+  if (m <= 0 || k <= 0 || ng <= kShortGroups || dtype == GNNREC_BF16) return 0;
+  return (dtype == GNNREC_F32 ? 3 : 2) * m * ng * kGroup * (int64_t)sizeof(bf16_t);
+}
+
 extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, const void* x,
                                 int64_t ldx, int64_t n, int64_t k, const void* codes,
-                                const void* scale, void* out, int64_t ldo,
+                                const void* scale, void* out, int64_t ldo, void* work,
                                 gnnrec_stream_t stream) {
   GNNREC_REQUIRE(dtype_ok(dtype) && dtype_ok(out_dtype), "q4_matmul: unknown dtype");
   const int rc = check_table("q4_matmul", n, k, codes, scale);
@@ -396,11 +564,29 @@ extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, con
                  (long long)m);
   if (n == 0 || m == 0) return GNNREC_OK;
   GNNREC_REQUIRE(x && out, "q4_matmul: null pointer");
-  const Q4Args p{m, ldx, n, k, ceil_div(k, kGroup), ldo, (const uint32_t*)codes,
-                 (const bf16_t*)scale, out, out_dtype};
+  GNNREC_REQUIRE(gnnrec_q4_matmul_work_bytes(dtype, m, k) == 0 || (work && aligned16(work)),
+                 "q4_matmul: the workspace is missing or not 16-B aligned");
+  const int64_t ng = ceil_div(k, kGroup);
+  const Q4Args p{m, n, k, ng, ldo, (const uint32_t*)codes, (const bf16_t*)scale, out, out_dtype};
+  const hipStream_t st = as_hip(stream);
   return with_dtype(dtype, [&](auto e) {
     using T = decltype(e);
-    return m <= 4 ? run_matmul<T, true>((const T*)x, p, as_hip(stream))
-                  : run_matmul<T, false>((const T*)x, p, as_hip(stream));
+    constexpr int kP = Parts<T>::n;
+    if (ng <= kShortGroups)
+      return m <= 4 ? run_short<T, true>((const T*)x, ldx, p, st)
+                    : run_short<T, false>((const T*)x, ldx, p, st);
+    const bf16_t* xs = (const bf16_t*)x;
+    int64_t lds = ldx, plane = 0;
+    if (kP > 1) {
+      const int64_t kp = ng * kGroup;
+      hipLaunchKernelGGL((split_users_kernel<T>),
+                         dim3((unsigned)ceil_div(m * (kp / 8), kQ4Block)), dim3(kQ4Block), 0, st,
+                         (const T*)x, ldx, m, k, kp, (bf16_t*)work);
+      const int rc2 = check_launch("q4_matmul (users)");
+      if (rc2 != GNNREC_OK) return rc2;
+      xs = (const bf16_t*)work, lds = kp, plane = m * kp;
+    }
+    return m <= 4 ? run_long<kP, true>(xs, lds, plane, p, st)
+                  : run_long<kP, false>(xs, lds, plane, p, st);
   });
 }

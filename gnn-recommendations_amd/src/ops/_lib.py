@@ -153,11 +153,13 @@ _SIGNATURES = {
                                    _i64, _p, _p, _p, _p],
     "gnnrec_quantize_q4": [_i32, _i64, _i64, _p, _i64, _p, _p, _p],
     "gnnrec_dequantize_q4": [_i64, _i64, _p, _p, _p, _i64, _p],
-    "gnnrec_q4_matmul": [_i32, _i32, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
+    "gnnrec_q4_matmul_work_bytes": [_i32, _i64, _i64],
+    "gnnrec_q4_matmul": [_i32, _i32, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p],
 }
 _RESTYPES = {"gnnrec_version": C.c_char_p, "gnnrec_last_error": C.c_char_p,
              "gnnrec_abi_version": C.c_int,
-             "gnnrec_layer_norm_work_floats": C.c_int64, "gnnrec_tiled_plan_device_scratch_words": C.c_int64}
+             "gnnrec_layer_norm_work_floats": C.c_int64,
+             "gnnrec_q4_matmul_work_bytes": C.c_int64, "gnnrec_tiled_plan_device_scratch_words": C.c_int64}
 
 EXPORTED = tuple(_SIGNATURES)
 

@@ -20,6 +20,7 @@ from ._lib import ptr
 from .rowwise import launch, rows_of
 
 GROUP = 32     # columns that share a scale; the kernels' matrix step is as deep
+SHORT_COLUMNS = 256     # up to here the users need no workspace (csrc/q4.hip kShortGroups)
 
 
 class Q4Table:
@@ -115,6 +116,12 @@ def q4_matmul(x: torch.Tensor, table: Q4Table,
     if m > 65535:
         raise NotImplementedError(f"q4_matmul: {m} rows of x, at most 65535")
     out = torch.empty((m, n) if x.dim() == 2 else (n,), dtype=out_dtype, device=x.device)
-    launch("gnnrec_q4_matmul", x.device, _lib.DTYPES[x.dtype], _lib.DTYPES[out_dtype], m,
-           ptr(x2), x2.stride(0), n, table.k, ptr(table.codes), ptr(table.scale), ptr(out), n)
+    t = _lib.DTYPES[x.dtype]
+    work = None
+    if table.k > SHORT_COLUMNS:
+        nbytes = _lib.lib().gnnrec_q4_matmul_work_bytes(t, m, table.k)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    launch("gnnrec_q4_matmul", x.device, t, _lib.DTYPES[out_dtype], m, x2.data_ptr(),
+           x2.stride(0), n, table.k, table.codes.data_ptr(), table.scale.data_ptr(),
+           out.data_ptr(), n, ptr(work))
     return out

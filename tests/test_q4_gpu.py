@@ -120,7 +120,7 @@ def test_output_rows_keep_their_neighbours(cuda):
     x = torch.randn(5, 64, device="cuda")
     out = torch.full((7, 90), 3.0, device="cuda")
     launch("gnnrec_q4_matmul", x.device, 0, 0, 5, x.data_ptr(), 64, 75, 64, t.codes.data_ptr(),
-           t.scale.data_ptr(), out.data_ptr(), 90)
+           t.scale.data_ptr(), out.data_ptr(), 90, None)
     assert (out[5:] == 3).all() and (out[:, 75:] == 3).all()
     assert torch.equal(out[:5, :75], ops.q4_matmul(x, t))
 

@@ -143,17 +143,20 @@ def test_c_entries_refuse_before_they_launch():
     assert L.gnnrec_layer_norm_work_floats(5, 64) == 2 * 64
     assert L.gnnrec_layer_norm_work_floats(0, 64) == 0
 
-    def q4(dtype=0, out=0, m=1, n=4, k=64, codes=a, x=a, o=a):
-        return _err(L.gnnrec_q4_matmul(dtype, out, m, x, k, n, k, codes, a, o, n, None))
+    def q4(dtype=0, out=0, m=1, n=4, k=64, codes=a, x=a, o=a, work=None):
+        return _err(L.gnnrec_q4_matmul(dtype, out, m, x, k, n, k, codes, a, o, n, work, None))
 
     for kw, word in ((dict(dtype=7), "dtype"), (dict(out=7), "dtype"), (dict(m=-1), "rows"),
                      (dict(m=65536), "65535"), (dict(n=-1), "size"), (dict(k=0), "size"),
                      (dict(k=2 ** 30), "size"), (dict(codes=None), "null"),
                      (dict(codes=a + 4), "aligned"), (dict(x=None), "null"),
-                     (dict(o=None), "null"), (dict(n=2 ** 50), "large")):
+                     (dict(o=None), "null"), (dict(n=2 ** 50), "large"),
+                     (dict(k=257), "workspace"), (dict(k=257, work=a + 4), "workspace")):
         rc, msg = q4(**kw)
         assert rc == -1 and word in msg, (kw, msg)
     assert q4(n=0)[0] == 0 and q4(m=0)[0] == 0
+    assert [L.gnnrec_q4_matmul_work_bytes(t, 5, k) for t in (0, 1, 2) for k in (256, 257)] \
+        == [0, 3 * 5 * 288 * 2, 0, 0, 0, 2 * 5 * 288 * 2]
     assert L.gnnrec_quantize_q4(0, 4, 64, None, 64, a, a, None) == -1
     assert L.gnnrec_quantize_q4(9, 4, 64, a, 64, a, a, None) == -1
     assert L.gnnrec_dequantize_q4(4, 64, a, a, None, 64, None) == -1
