@@ -152,36 +152,16 @@ __device__ __forceinline__ uint32_t cut(float& v) {
   return top;
 }
 
-// A's fragments of one group: eight values x[user, c ..] of this lane, cut into parts.
-template <class T, bool FEW>
-__device__ __forceinline__ void load_users(const T* __restrict__ row, bool valid, int part,
-                                           int64_t c, int64_t k,
-                                           bf16x8 (&a)[FEW ? 1 : Parts<T>::n]) {
-  constexpr int kP = Parts<T>::n;
-  float v[8];
-  load8(row + c, valid ? k - c : 0, v);
-  uint32_t bits[kP][8];
+// Eight values cut into their bf16 parts.
+template <int P>
+__device__ __forceinline__ void split8(float (&v)[8], u32x4 (&parts)[P]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-#pragma unroll
-    for (int i = 0; i < kP; ++i) bits[i][e] = cut(v[e]);
-#pragma unroll
-  for (int i = 0; i < (FEW ? 1 : kP); ++i) {
-    u32x4 w;
+  for (int i = 0; i < P; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      uint32_t lo = bits[i][2 * e], hi = bits[i][2 * e + 1];
-      if (FEW) {
-#pragma unroll
-        for (int j = 1; j < kP; ++j) {
-          lo = part == j ? bits[j][2 * e] : lo;
-          hi = part == j ? bits[j][2 * e + 1] : hi;
-        }
-      }
-      w[e] = (lo >> 16) | hi;
+      const uint32_t lo = cut(v[2 * e]), hi = cut(v[2 * e + 1]);
+      parts[i][e] = (lo >> 16) | hi;
     }
-    a[i] = __builtin_bit_cast(bf16x8, w);
-  }
 }
 
 __device__ __forceinline__ void store_out(void* out, int32_t dtype, int64_t i, float v) {
@@ -198,90 +178,94 @@ struct Q4Args {
   int32_t out_dtype;
 };
 
-// acc[t] += the products of R groups from g0 on (R == 4: as many of four as the row has) of NT
-// tiles of 16 items. Rows are given as an offset from `base`, clamped to the table's last row (a
-// clamped row's results are not stored).
+// Codes and scales of R groups from g0 on (R == 4: as many of four as the row has) of NT tiles of
+// 16 items, in flight. Rows are offsets from `base`, clamped to the table's last row, and groups
+// to the row's last one, so every load is unconditional and within the table; what a clamped
+// load brings is not used (a tile's results depend on their own row alone).
 //
-// Loads: with four groups, lane (q, r) takes 16 bytes, group g0 + q of row r of a tile; of rows
-// with only two (one) groups left, a load covers two (four) tiles, so that no lane idles and the
-// wave reads one contiguous piece. Either way word j of load i after the transposition holds
-// eight codes of one (tile, group) in every lane row. Scales: lane l takes those of row l of the
-// 64, and two swaps spread a tile's to all lane rows.
-template <int NT, int R, int KA, class A>
-__device__ __forceinline__ void groups(const Q4Args& p, int64_t base, int64_t g0, A&& users,
-                                       f32x4 (&acc)[NT]) {
-  static_assert(NT == 4 || (NT == 1 && R == 4), "a single tile always takes four groups");
-  constexpr int kLoads = NT == 4 ? R : 1;  // four tiles x R groups, four pieces of 16 B a load
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int last = (int)(p.n - 1 - base < 63 ? p.n - 1 - base : 63);
-  const uint32_t* codes = p.codes + (base * p.ng + g0) * 4;
-  const uint16_t* scale = reinterpret_cast<const uint16_t*>(p.scale) + base * p.ng + g0;
-  const int here = p.ng - g0 < 4 ? (int)(p.ng - g0) : 4;  // groups left
+// With four groups, lane (q, r) takes 16 bytes, group g0 + q of row r of a tile; of rows with only
+// two (one) groups, a load covers two (four) tiles, so that no lane idles and the wave reads one
+// contiguous piece. Either way word j of load i after the transposition holds eight codes of one
+// (tile, group) in every lane row. Scales: lane l takes those of row l of the 64.
+template <int NT, int R>
+struct Codes {
+  // NT tiles x R groups, four 16-B pieces a load (of one or two tiles always four groups)
+  static constexpr int kLoads = NT == 4 ? R : NT;
   u32x4 w[kLoads];
+  uint32_t s[2];  // s[h]: scales of groups g0 + 2 h and g0 + 2 h + 1
+
+  __device__ __forceinline__ void load(const Q4Args& p, int64_t base, int64_t g0) {
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int last = (int)(p.n - 1 - base < 63 ? p.n - 1 - base : 63);
+    const int end = p.ng - g0 < 4 ? (int)(p.ng - g0) - 1 : 3;  // the last group of these
+    const uint32_t* codes = p.codes + (base * p.ng + g0) * 4;
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int row = (R == 4 ? i * 16 : R == 2 ? i * 32 + (q >> 1) * 16 : q * 16) + r;
-    const int g = R == 4 ? q : R == 2 ? (q & 1) : 0;
-    w[i] = u32x4{0, 0, 0, 0};
-    if (R < 4 || g < here)
-      w[i] = *reinterpret_cast<const u32x4*>(
-          codes + ((int64_t)(row < last ? row : last) * p.ng + g) * 4);
-  }
-  // s[h]: scales of groups g0 + 2 h and g0 + 2 h + 1
-  uint32_t s[2] = {0, 0};
-  {
-    const int row = NT == 4 ? lane : r;
-    const uint16_t* at = scale + (int64_t)(row < last ? row : last) * p.ng;
-    struct __attribute__((packed)) Two { uint32_t v[2]; };
-    struct __attribute__((packed)) One { uint32_t v; };
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = (R == 4 ? i * 16 : R == 2 ? i * 32 + (q >> 1) * 16 : q * 16) + r;
+      const int g = R == 4 ? min(q, end) : R == 2 ? (q & 1) : 0;
+      w[i] = *reinterpret_cast<const u32x4*>(codes + ((int64_t)min(row, last) * p.ng + g) * 4);
+    }
+    struct __attribute__((packed)) Pair { uint32_t v; };
+    const int row = min(lane & (NT * 16 - 1), last);
+    const uint16_t* at = reinterpret_cast<const uint16_t*>(p.scale) + (base + row) * p.ng + g0;
     if (R == 1) {
       s[0] = at[0];
-    } else if (R == 2) {
-      s[0] = reinterpret_cast<const One*>(at)->v;
-    } else if (here == 4) {
-      const Two v = *reinterpret_cast<const Two*>(at);
-      s[0] = v.v[0], s[1] = v.v[1];
-    } else {
-      s[0] = at[0];
-      if (here > 1) s[0] |= (uint32_t)at[1] << 16;
-      if (here > 2) s[1] = at[2];
+    } else {  // two at a time; a pair that would leave the row is read one earlier
+      const int back0 = R == 4 && end < 1, back1 = R == 4 ? max(0, 3 - end) : 0;
+      s[0] = reinterpret_cast<const Pair*>(at - back0)->v >> (16 * back0);
+      if (R == 4) {
+        const int o = max(2 - back1, end > 0 ? 0 : -1);
+        s[1] = reinterpret_cast<const Pair*>(at + o)->v >> (16 * min(back1, 1));
+      }
     }
   }
-  uint32_t st[2][4];
+
+  // acc[t] += the products with users(g), the fragments of group g0 + g.
+  template <int KA, class A>
+  __device__ __forceinline__ void multiply(int64_t left, A&& users, f32x4 (&acc)[NT]) {
+    uint32_t st[2][4];
 #pragma unroll
-  for (int h = 0; h < (R == 4 ? 2 : 1); ++h) {
-    if (NT == 1) {
-      st[h][0] = s[h];
-    } else {
-      uint32_t a = s[h], b = s[h];
-      swap16(a, b);  // rows (0 0 2 2) and (1 1 3 3)
-      uint32_t c = a, d = b;
-      swap32(a, c);
-      swap32(b, d);
-      st[h][0] = a, st[h][1] = b, st[h][2] = c, st[h][3] = d;
+    for (int h = 0; h < (R == 4 ? 2 : 1); ++h) {
+      if (NT == 1) {
+        st[h][0] = s[h];
+      } else if (NT == 2) {
+        uint32_t a = s[h], b = s[h];  // rows (0 1 0 1)
+        swap16(a, b);
+        st[h][0] = a, st[h][1] = b;
+      } else {  // a tile's scales to all lane rows
+        uint32_t a = s[h], b = s[h];
+        swap16(a, b);  // rows (0 0 2 2) and (1 1 3 3)
+        uint32_t c = a, d = b;
+        swap32(a, c);
+        swap32(b, d);
+        st[h][0] = a, st[h][1] = b, st[h][2] = c, st[h][3] = d;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) transpose4(w[i]);
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+      if (R == 4 && g >= left) break;
+      bf16x8 a[KA];
+      users(g, a);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint32_t word = R == 4 ? w[t][g] : R == 2 ? w[t >> 1][(t & 1) * 2 + g] : w[0][t];
+        const bf16x8 bf = codes_to_bf16(word);
+        f32x4 d = {};
+#pragma unroll
+        for (int i = KA - 1; i >= 0; --i)
+          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], bf, d, 0, 0, 0);
+        const uint32_t sw = st[g >> 1][t];
+        const float sc = __uint_as_float(g & 1 ? sw & 0xffff0000u : sw << 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(sc, d[i], acc[t][i]);
+      }
+      // one group at a time: all four together would take twice the registers and half the waves
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) transpose4(w[i]);
-#pragma unroll
-  for (int g = 0; g < R; ++g) {
-    if (R == 4 && g >= here) break;
-    const auto& a = users(g);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const uint32_t word = R == 4 ? w[t][g] : R == 2 ? w[t >> 1][(t & 1) * 2 + g] : w[0][t];
-      const bf16x8 bf = codes_to_bf16(word);
-      f32x4 d = {};
-#pragma unroll
-      for (int i = KA - 1; i >= 0; --i)
-        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], bf, d, 0, 0, 0);
-      const uint32_t sw = st[g >> 1][t];
-      const float sc = __uint_as_float(g & 1 ? sw & 0xffff0000u : sw << 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(sc, d[i], acc[t][i]);
-    }
-  }
-}
+};
 
 // The results of NT tiles. Lane (q, r) holds users 4 q + i of item r of a tile, or part q of user
 // i; a transposition gives a register 64 neighbouring items of one user (NT == 4), or the parts
@@ -314,118 +298,210 @@ __device__ __forceinline__ void store_tiles(const Q4Args& p, int64_t base, int64
       }
     }
   } else {
-    const int64_t item = base + r;
-    if (FEW) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int64_t item = base + t * 16 + r;
       u32x4 v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(acc[0][i]);
-      transpose4(v);
-      float s = __uint_as_float(v[0]);
+      for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(acc[t][i]);
+      if (FEW) {
+        transpose4(v);
+        float s = __uint_as_float(v[0]);
 #pragma unroll
-      for (int j = 1; j < PARTS; ++j) s += __uint_as_float(v[j]);
-      if (user0 + q < p.m && item < p.n)
-        store_out(p.out, p.out_dtype, (user0 + q) * p.ldo + item, s);
-    } else {
+        for (int j = 1; j < PARTS; ++j) s += __uint_as_float(v[j]);
+        if (user0 + q < p.m && item < p.n)
+          store_out(p.out, p.out_dtype, (user0 + q) * p.ldo + item, s);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t u = user0 + 4 * q + i;
-        if (u < p.m && item < p.n) store_out(p.out, p.out_dtype, u * p.ldo + item, acc[0][i]);
-      }
-    }
-  }
-}
-
-// Short rows (at most 8 groups, 256 columns): the users' fragments stay in registers over all the
-// items of a wave. FEW: at most four users a tile, the parts in the instruction's idle rows. HELD
-// steps of four groups, the last of R.
-template <class T, bool FEW, int NT, int HELD, int R>
-__global__ __launch_bounds__(kQ4Block) void q4_short_kernel(const T* __restrict__ x, int64_t ldx,
-                                                            Q4Args p) {
-  constexpr int kA = FEW ? 1 : Parts<T>::n;
-  constexpr int kHeld = (HELD - 1) * 4 + R;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int r = lane & 15, q = lane >> 4;
-  const int64_t user0 = (int64_t)blockIdx.y * (FEW ? 4 : 16);
-  const int64_t user = user0 + (FEW ? (r & 3) : r);
-  const int part = FEW ? r >> 2 : 0;
-  const bool valid = user < p.m && part < Parts<T>::n;
-  bf16x8 held[kHeld][kA];
-#pragma unroll
-  for (int g = 0; g < kHeld; ++g)
-    load_users<T, FEW>(x + (valid ? user : 0) * ldx, valid, part, (int64_t)g * kGroup + q * 8, p.k,
-                       held[g]);
-  const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16);
-  for (int64_t task = (int64_t)blockIdx.x * 4 + wave; task < tasks; task += (int64_t)gridDim.x * 4) {
-    const int64_t base = task * NT * 16;
-    f32x4 acc[NT] = {};
-    if (HELD == 2)
-      groups<NT, 4, kA>(p, base, 0, [&](int g) -> auto& { return held[g % kHeld]; }, acc);
-    groups<NT, R, kA>(p, base, (HELD - 1) * 4,
-                      [&](int g) -> auto& { return held[(HELD - 1) * 4 + g]; }, acc);
-    store_tiles<FEW, NT, Parts<T>::n>(p, base, user0, acc);
-  }
-}
-
-// Long rows: the users come as bf16 parts (plane i at x + i * plane, rows ldx apart), from the
-// table itself or from split_users_kernel. WK waves share a tile set and split its groups; their
-// sums are joined through LDS in the waves' order.
-template <int PARTS, bool FEW, int NT, int WK>
-__global__ __launch_bounds__(WK > 4 ? WK * 64 : 256) void q4_long_kernel(
-    const bf16_t* __restrict__ x, int64_t ldx, int64_t plane, Q4Args p) {
-  constexpr int kA = FEW ? 1 : PARTS;
-  __shared__ f32x4 join[WK > 1 ? (WK - 1) * NT * 64 : 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int r = lane & 15, q = lane >> 4;
-  const int64_t user0 = (int64_t)blockIdx.y * (FEW ? 4 : 16);
-  const int64_t user = user0 + (FEW ? (r & 3) : r);
-  const int part = FEW ? r >> 2 : 0;
-  const bool valid = user < p.m && part < PARTS;
-  const bf16_t* xrow = x + (valid ? part * plane + user * ldx : 0);
-  const int64_t blocks4 = (p.ng + 3) >> 2;
-  const int64_t b0 = WK > 1 ? blocks4 * wave / WK : 0;
-  const int64_t b1 = WK > 1 ? blocks4 * (wave + 1) / WK : blocks4;
-  const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16);
-  const int64_t first = WK > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  const int64_t step = WK > 1 ? gridDim.x : (int64_t)gridDim.x * 4;
-  for (int64_t task = first; task < tasks; task += step) {
-    const int64_t base = task * NT * 16;
-    f32x4 acc[NT] = {};
-#pragma unroll 2
-    for (int64_t b = b0; b < b1; ++b) {
-      bf16x8 a[4][kA];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int64_t c = (b * 4 + g) * kGroup + q * 8;
-#pragma unroll
-        for (int i = 0; i < kA; ++i) {
-          a[g][i] = bf16x8{};
-          if (valid && c + 8 <= p.k) {
-            a[g][i] = __builtin_bit_cast(
-                bf16x8, *reinterpret_cast<const Eight<bf16_t>*>(xrow + i * plane + c));
-          } else if (valid && c < p.k) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (c + e < p.k) a[g][i][e] = xrow[i * plane + c + e];
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int64_t u = user0 + 4 * q + i;
+          if (u < p.m && item < p.n)
+            store_out(p.out, p.out_dtype, u * p.ldo + item, __uint_as_float(v[i]));
         }
       }
-      groups<NT, 4, kA>(p, base, b * 4, [&](int g) -> auto& { return a[g]; }, acc);
     }
-    if (WK > 1) {
-      if (wave > 0) {
+  }
+}
+
+// Many items or short rows: the workgroup cuts its users into fragments once, all groups of them,
+// in LDS, and its waves walk tile sets of their own, the codes one step (four groups, or R) ahead
+// through the end of a tile set into the next. FEW: at most four users a tile, their parts in the
+// instruction's idle rows.
+template <class T, bool FEW, int NT, int R>
+__global__ __launch_bounds__(kQ4Block, FEW ? 4 : 3) void q4_walk_kernel(const T* __restrict__ x,
+                                                                        int64_t ldx, Q4Args p) {
+  constexpr int kP = Parts<T>::n, kA = FEW ? 1 : kP, kUsers = FEW ? 4 : 16;
+  extern __shared__ u32x4 frag[];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t user0 = (int64_t)blockIdx.y * kUsers;
+  const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16), stride = (int64_t)gridDim.x * 4;
+  const int64_t steps = R == 4 ? (p.ng + 3) >> 2 : 1;
+  int64_t task = (int64_t)blockIdx.x * 4 + wave;
+  Codes<NT, R> now, next;
+  if (task < tasks) now.load(p, task * NT * 16, 0);
+  // rows of A that no user fills are left as they are: they reach no result that is stored
+  const int users = (int)(p.m - user0 < kUsers ? p.m - user0 : kUsers), per = (int)p.ng * 4;
+  for (int i = threadIdx.x; i < users * per; i += kQ4Block) {
+    const int u = i / per, c = i - u * per;
+    float v[8];
+    load8(x + (user0 + u) * ldx + c * 8, p.k - c * 8, v);
+    u32x4 parts[kP];
+    split8(v, parts);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) join[((wave - 1) * NT + t) * 64 + lane] = acc[t];
-      }
-      __syncthreads();
-      if (wave == 0) {
-        for (int v = 0; v < WK - 1; ++v)
+    for (int j = 0; j < kP; ++j)
+      frag[((c >> 2) * kA + (FEW ? 0 : j)) * 64 + (c & 3) * 16 + (FEW ? j * 4 + u : u)] = parts[j];
+  }
+  __syncthreads();
+  while (task < tasks) {
+    f32x4 acc[NT] = {};
+    const int64_t base = task * NT * 16;
+    task += stride;
+    for (int64_t b = 0; b < steps; ++b) {
+      if (b + 1 < steps) next.load(p, base, (b + 1) * 4);
+      else if (task < tasks) next.load(p, task * NT * 16, 0);
+      now.template multiply<kA>(
+          p.ng - b * 4,
+          [&](int g, bf16x8(&a)[kA]) {
 #pragma unroll
-          for (int t = 0; t < NT; ++t) acc[t] += join[(v * NT + t) * 64 + lane];
-      }
-      __syncthreads();  // the sums have been read before the next task's are written
-      if (wave > 0) continue;
+            for (int i = 0; i < kA; ++i)
+              a[i] = __builtin_bit_cast(bf16x8, frag[((b * 4 + g) * kA + i) * 64 + lane]);
+          },
+          acc);
+      now = next;
     }
-    store_tiles<FEW, NT, PARTS>(p, base, user0, acc);
+    store_tiles<FEW, NT, kP>(p, base, user0, acc);
+  }
+}
+
+// The sums of a tile set over the WK waves that split its groups, in wave 0, in the waves' order.
+template <int NT, int WK>
+__device__ __forceinline__ void join_waves(f32x4 (&acc)[NT], f32x4* join) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave > 0) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) join[((wave - 1) * NT + t) * 64 + lane] = acc[t];
+  }
+  __syncthreads();
+  if (wave == 0) {
+    for (int v = 0; v < WK - 1; ++v)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] += join[(v * NT + t) * 64 + lane];
+  }
+  __syncthreads();  // the sums have been read before the next tile set's are written
+}
+
+// Long rows, at most four users a tile: WK waves share a tile set and split its groups, STEPS
+// steps of four groups in flight. The workgroup keeps the users' parts in LDS, row j * users + u
+// padded by 64 B, cut while the first codes are on their way.
+template <class T, int NT, int WK, int STEPS>
+__global__ __launch_bounds__(WK * 64, 4) void q4_few_kernel(const T* __restrict__ x, int64_t ldx,
+                                                         Q4Args p) {
+  constexpr int kP = Parts<T>::n;
+  extern __shared__ u32x4 rows[];
+  __shared__ f32x4 join[(WK - 1) * NT * 64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const int64_t user0 = (int64_t)blockIdx.y * 4;
+  const int users = (int)(p.m - user0 < 4 ? p.m - user0 : 4);
+  const int per = (int)p.ng * 4, pitch = per + 4;  // 16-B pieces
+  const int64_t steps = (p.ng + 3) >> 2;
+  const int64_t b0 = steps * wave / WK, b1 = steps * (wave + 1) / WK;
+  const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16);
+  // rows of A that no user fills repeat another's: they reach no result that is stored
+  const int mine = (min(r >> 2, kP - 1) * users + min(r & 3, users - 1)) * pitch + q;
+  Codes<NT, 4> now[STEPS];
+  auto load = [&](int64_t task, int64_t b) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      now[i].load(p, task * NT * 16, (b + i < steps ? b + i : steps - 1) * 4);
+  };
+  load(blockIdx.x, b0);
+  for (int u = 0; u < users; ++u)
+    for (int c = threadIdx.x; c < per; c += WK * 64) {
+      float v[8];
+      load8(x + (user0 + u) * ldx + c * 8, p.k - c * 8, v);
+      u32x4 parts[kP];
+      split8(v, parts);
+#pragma unroll
+      for (int j = 0; j < kP; ++j) rows[(j * users + u) * pitch + c] = parts[j];
+    }
+  __syncthreads();
+  for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
+    f32x4 acc[NT] = {};
+    if (task != blockIdx.x) load(task, b0);
+    for (int64_t b = b0;;) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        if (b + i >= b1) break;
+        now[i].template multiply<1>(
+            p.ng - (b + i) * 4,
+            [&](int g, bf16x8(&f)[1]) {
+              f[0] = __builtin_bit_cast(bf16x8, rows[mine + ((b + i) * 4 + g) * 4]);
+            },
+            acc);
+      }
+      b += STEPS;
+      if (b >= b1) break;
+      load(task, b);
+    }
+    join_waves<NT, WK>(acc, join);
+    if (wave == 0) store_tiles<true, NT, kP>(p, task * NT * 16, user0, acc);
+  }
+}
+
+// Long rows, more users: they come as bf16 parts in rows of whole groups (plane i at x + i *
+// plane, rows ldx apart), from the table itself or from split_users_kernel, and a step's
+// fragments (1 KB a group and part) are loaded from the caches with its codes, one step ahead.
+template <int PARTS, int NT, int WK>
+__global__ __launch_bounds__(WK * 64, 2) void q4_many_kernel(const bf16_t* __restrict__ x,
+                                                          int64_t ldx, int64_t plane, Q4Args p) {
+  __shared__ f32x4 join[(WK - 1) * NT * 64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const int64_t user0 = (int64_t)blockIdx.y * 16;
+  const bf16_t* xrow = x + (user0 + r < p.m ? user0 + r : p.m - 1) * ldx + q * 8;
+  const int64_t steps = (p.ng + 3) >> 2;
+  const int64_t b0 = steps * wave / WK, b1 = steps * (wave + 1) / WK;
+  const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16);
+  struct Step {
+    Codes<NT, 4> codes;
+    bf16x8 a[4][PARTS];
+  };
+  for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const int64_t base = task * NT * 16;
+    auto load = [&](Step& s, int64_t b) {
+      b = b < steps ? b : steps - 1;
+      s.codes.load(p, base, b * 4);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int64_t at = b * 4 + g < p.ng ? b * 4 + g : p.ng - 1;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+          s.a[g][i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const Eight<bf16_t>*>(
+                                                     xrow + i * plane + at * kGroup));
+      }
+    };
+    auto multiply = [&](Step& s, int64_t b, f32x4(&acc)[NT]) {
+      s.codes.template multiply<PARTS>(
+          p.ng - b * 4,
+          [&](int g, bf16x8(&f)[PARTS]) {
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) f[i] = s.a[g][i];
+          },
+          acc);
+    };
+    f32x4 acc[NT] = {};
+    Step one, two;
+    load(one, b0);
+    for (int64_t b = b0; b < b1; b += 2) {
+      if (b + 1 < b1) load(two, b + 1);
+      multiply(one, b, acc);
+      if (b + 1 >= b1) break;
+      if (b + 2 < b1) load(one, b + 2);
+      multiply(two, b + 1, acc);
+    }
+    join_waves<NT, WK>(acc, join);
+    if (wave == 0) store_tiles<false, NT, PARTS>(p, base, user0, acc);
   }
 }
 
@@ -441,67 +517,98 @@ __global__ __launch_bounds__(kQ4Block) void split_users_kernel(const T* __restri
   if (row >= m) return;
   float v[8];
   load8(x + row * ldx + c, k - c, v);
+  u32x4 w[kP];
+  split8(v, w);
 #pragma unroll
-  for (int j = 0; j < kP; ++j) {
-    u32x4 w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t lo = cut(v[2 * e]), hi = cut(v[2 * e + 1]);
-      w[e] = (lo >> 16) | hi;
-    }
-    *reinterpret_cast<u32x4*>(parts + (j * m + row) * kp + c) = w;
-  }
+  for (int j = 0; j < kP; ++j) *reinterpret_cast<u32x4*>(parts + (j * m + row) * kp + c) = w[j];
 }
 
-constexpr int64_t kShortGroups = 8;
+// Workgroups of a walk (three a CU are resident; with several user tiles each takes fewer, as the
+// tiles share the codes in the caches) and of the split products. 16 users x 1M x 64 fp32: 768
+// 20.7 us, 1024 23.8, 2048 25.2; 64 users: 384 a tile 72.0, 256 82.8, 512 75.8.
+constexpr int64_t kWalkGrid = 768, kWalkGridTiled = 384, kSplitGrid = 1024;
+// LDS that the users' fragments or rows may take: two workgroups still fit a CU (160 KB), and
+// with the joined sums the rows stay below 64 KB.
+constexpr int64_t kWalkBytes = 64 * 1024, kFewBytes = 48 * 1024;
+// Items from which waves walk long rows alone (125 000 x 512, one user: 13.1 us, split 49.3), and
+// from which a tile set is four tiles (4 users x 30 000 x 1 000: one tile 10.7 us, four 14.9).
+constexpr int64_t kManyItems = 16384, kWideItems = 65536;
+
+static int64_t parts_of(int32_t dtype) {
+  return dtype == GNNREC_F32 ? 3 : dtype == GNNREC_F16 ? 2 : 1;
+}
+
+// How a product is shared out.
+//  walk: a wave walks whole rows; needs all groups' fragments of a user tile in LDS (1 KB a group,
+//        and for more than four users a part), and either rows of at most 256 columns (then also
+//        few items are quick) or items for all waves.
+//  few:  the waves of a workgroup split long rows; at most four users, whose parts fit LDS.
+//  many: the same with the fragments from the caches; the rest.
+enum class Q4Plan { walk, few, many };
+static int64_t few_bytes(int32_t dtype, int64_t m, int64_t ng) {
+  return (m < 4 ? m : 4) * parts_of(dtype) * (ng * 4 + 4) * 16;
+}
+static int64_t walk_bytes(int32_t dtype, int64_t m, int64_t ng) {
+  return ng * (m <= 4 ? 1 : parts_of(dtype)) * 1024;
+}
+static Q4Plan plan_of(int32_t dtype, int64_t m, int64_t n, int64_t ng) {
+  if (walk_bytes(dtype, m, ng) <= kWalkBytes && (ng <= 8 || n >= kManyItems)) return Q4Plan::walk;
+  return m <= 4 && few_bytes(dtype, m, ng) <= kFewBytes ? Q4Plan::few : Q4Plan::many;
+}
 
 template <class T, bool FEW>
-static int run_short(const T* x, int64_t ldx, const Q4Args& p, hipStream_t stream) {
-  auto go = [&](auto nt, auto held, auto rem) {
+static int run_walk(int32_t dtype, const T* x, int64_t ldx, const Q4Args& p, hipStream_t stream) {
+  auto go = [&](auto nt, auto rem) {
+    const int64_t tiles = ceil_div(p.m, FEW ? 4 : 16);
+    const int64_t most = tiles == 1 ? kWalkGrid : kWalkGridTiled;
     const int64_t want = ceil_div(ceil_div(p.n, nt.value * 16), 4);
-    hipLaunchKernelGGL((q4_short_kernel<T, FEW, nt.value, held.value, rem.value>),
-                       dim3((unsigned)(want < 2048 ? want : 2048),
-                            (unsigned)ceil_div(p.m, FEW ? 4 : 16)),
-                       dim3(kQ4Block), 0, stream, x, ldx, p);
+    hipLaunchKernelGGL((q4_walk_kernel<T, FEW, nt.value, rem.value>),
+                       dim3((unsigned)(want < most ? want : most), (unsigned)tiles),
+                       dim3(kQ4Block), walk_bytes(dtype, p.m, p.ng), stream, x, ldx, p);
     return check_launch("q4_matmul");
   };
   using std::integral_constant;
   const integral_constant<int, 1> i1{};
   const integral_constant<int, 2> i2{};
   const integral_constant<int, 4> i4{};
-  if (p.n < 64 * 1024) {  // one tile a wave: four times the waves
-    if (p.ng <= 4) return go(i1, i1, i4);
-    return go(i1, i2, i4);
-  }
-  switch (p.ng) {
-    case 1: return go(i4, i1, i1);
-    case 2: return go(i4, i1, i2);
-    case 3: case 4: return go(i4, i1, i4);
-    case 5: return go(i4, i2, i1);
-    case 6: return go(i4, i2, i2);
-    default: return go(i4, i2, i4);
-  }
+  if (p.n < kWideItems) return p.ng == 1 ? go(i1, i1) : go(i1, i4);  // four times the waves
+  return p.ng == 1 ? go(i4, i1) : p.ng == 2 ? go(i4, i2) : go(i4, i4);
 }
 
-template <int PARTS, bool FEW>
-static int run_long(const bf16_t* x, int64_t ldx, int64_t plane, const Q4Args& p,
-                    hipStream_t stream) {
-  auto go = [&](auto nt, auto wk) {
+template <class T>
+static int run_few(int32_t dtype, const T* x, int64_t ldx, const Q4Args& p, hipStream_t stream) {
+  auto go = [&](auto nt, auto wk, auto steps) {
     const int64_t tasks = ceil_div(p.n, nt.value * 16);
-    const int64_t want = wk.value == 1 ? ceil_div(tasks, 4) : tasks;
-    hipLaunchKernelGGL((q4_long_kernel<PARTS, FEW, nt.value, wk.value>),
-                       dim3((unsigned)(want < 4096 ? want : 4096),
-                            (unsigned)ceil_div(p.m, FEW ? 4 : 16)),
-                       dim3(wk.value > 4 ? wk.value * 64 : 256), 0, stream, x, ldx, plane, p);
+    hipLaunchKernelGGL((q4_few_kernel<T, nt.value, wk.value, steps.value>),
+                       dim3((unsigned)(tasks < kSplitGrid ? tasks : kSplitGrid),
+                            (unsigned)ceil_div(p.m, 4)),
+                       dim3(wk.value * 64), few_bytes(dtype, p.m, p.ng), stream, x, ldx, p);
     return check_launch("q4_matmul");
   };
   using std::integral_constant;
   const integral_constant<int, 1> i1{};
   const integral_constant<int, 4> i4{};
   const integral_constant<int, 8> i8{};
-  if (p.n >= 64 * 4096) return go(i4, i1);
-  if (p.n >= 64 * 512) return go(i4, i4);
-  return p.ng >= 32 ? go(i1, i8) : go(i1, i4);
+  if (p.n >= kManyItems) return go(i4, i4, i1);
+  return p.ng >= 128 ? go(i1, i8, i4) : go(i1, i4, i4);
+}
+
+template <int PARTS>
+static int run_many(const bf16_t* x, int64_t ldx, int64_t plane, const Q4Args& p,
+                    hipStream_t stream) {
+  auto go = [&](auto nt, auto wk) {
+    const int64_t tasks = ceil_div(p.n, nt.value * 16);
+    hipLaunchKernelGGL((q4_many_kernel<PARTS, nt.value, wk.value>),
+                       dim3((unsigned)(tasks < kSplitGrid ? tasks : kSplitGrid),
+                            (unsigned)ceil_div(p.m, 16)),
+                       dim3(wk.value * 64), 0, stream, x, ldx, plane, p);
+    return check_launch("q4_matmul");
+  };
+  using std::integral_constant;
+  const integral_constant<int, 2> i2{};
+  const integral_constant<int, 4> i4{};
+  const integral_constant<int, 8> i8{};
+  return p.n >= kManyItems || p.ng < 128 ? go(i4, i4) : go(i2, i8);
 }
 
 static int check_table(const char* what, int64_t n, int64_t k, const void* codes,
@@ -547,10 +654,12 @@ extern "C" int gnnrec_dequantize_q4(int64_t n, int64_t k, const void* codes, con
   return check_launch("dequantize_q4");
 }
 
-extern "C" int64_t gnnrec_q4_matmul_work_bytes(int32_t dtype, int64_t m, int64_t k) {
+extern "C" int64_t gnnrec_q4_matmul_work_bytes(int32_t dtype, int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0 || !dtype_ok(dtype)) return 0;
   const int64_t ng = ceil_div(k, kGroup);
-  if (m <= 0 || k <= 0 || ng <= kShortGroups || dtype == GNNREC_BF16) return 0;
-  return (dtype == GNNREC_F32 ? 3 : 2) * m * ng * kGroup * (int64_t)sizeof(bf16_t);
+  if (plan_of(dtype, m, n, ng) != Q4Plan::many) return 0;
+  if (dtype == GNNREC_BF16 && k % kGroup == 0) return 0;  // x itself is read
+  return parts_of(dtype) * m * ng * kGroup * (int64_t)sizeof(bf16_t);
 }
 
 extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, const void* x,
@@ -564,7 +673,7 @@ extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, con
                  (long long)m);
   if (n == 0 || m == 0) return GNNREC_OK;
   GNNREC_REQUIRE(x && out, "q4_matmul: null pointer");
-  GNNREC_REQUIRE(gnnrec_q4_matmul_work_bytes(dtype, m, k) == 0 || (work && aligned16(work)),
+  GNNREC_REQUIRE(gnnrec_q4_matmul_work_bytes(dtype, m, n, k) == 0 || (work && aligned16(work)),
                  "q4_matmul: the workspace is missing or not 16-B aligned");
   const int64_t ng = ceil_div(k, kGroup);
   const Q4Args p{m, n, k, ng, ldo, (const uint32_t*)codes, (const bf16_t*)scale, out, out_dtype};
@@ -572,12 +681,14 @@ extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, con
   return with_dtype(dtype, [&](auto e) {
     using T = decltype(e);
     constexpr int kP = Parts<T>::n;
-    if (ng <= kShortGroups)
-      return m <= 4 ? run_short<T, true>((const T*)x, ldx, p, st)
-                    : run_short<T, false>((const T*)x, ldx, p, st);
+    const Q4Plan plan = plan_of(dtype, m, n, ng);
+    if (plan == Q4Plan::walk)
+      return m <= 4 ? run_walk<T, true>(dtype, (const T*)x, ldx, p, st)
+                    : run_walk<T, false>(dtype, (const T*)x, ldx, p, st);
+    if (plan == Q4Plan::few) return run_few<T>(dtype, (const T*)x, ldx, p, st);
     const bf16_t* xs = (const bf16_t*)x;
     int64_t lds = ldx, plane = 0;
-    if (kP > 1) {
+    if (kP > 1 || k % kGroup) {
       const int64_t kp = ng * kGroup;
       hipLaunchKernelGGL((split_users_kernel<T>),
                          dim3((unsigned)ceil_div(m * (kp / 8), kQ4Block)), dim3(kQ4Block), 0, st,
@@ -586,7 +697,6 @@ extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, con
       if (rc2 != GNNREC_OK) return rc2;
       xs = (const bf16_t*)work, lds = kp, plane = m * kp;
     }
-    return m <= 4 ? run_long<kP, true>(xs, lds, plane, p, st)
-                  : run_long<kP, false>(xs, lds, plane, p, st);
+    return run_many<kP>(xs, lds, plane, p, st);
   });
 }

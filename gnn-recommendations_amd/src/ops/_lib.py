@@ -153,7 +153,7 @@ _SIGNATURES = {
                                    _i64, _p, _p, _p, _p],
     "gnnrec_quantize_q4": [_i32, _i64, _i64, _p, _i64, _p, _p, _p],
     "gnnrec_dequantize_q4": [_i64, _i64, _p, _p, _p, _i64, _p],
-    "gnnrec_q4_matmul_work_bytes": [_i32, _i64, _i64],
+    "gnnrec_q4_matmul_work_bytes": [_i32, _i64, _i64, _i64],
     "gnnrec_q4_matmul": [_i32, _i32, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p],
 }
 _RESTYPES = {"gnnrec_version": C.c_char_p, "gnnrec_last_error": C.c_char_p,

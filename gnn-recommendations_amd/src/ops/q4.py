@@ -20,7 +20,7 @@ from ._lib import ptr
 from .rowwise import launch, rows_of
 
 GROUP = 32     # columns that share a scale; the kernels' matrix step is as deep
-SHORT_COLUMNS = 256     # up to here the users need no workspace (csrc/q4.hip kShortGroups)
+SHORT_COLUMNS = 256     # up to here the users need no workspace (csrc/q4.hip plan_of)
 
 
 class Q4Table:
@@ -28,6 +28,8 @@ class Q4Table:
     `scale` may have fewer columns, one for each `group` columns (a multiple of 32): it is
     repeated here once. The tensors are kept, not copied; what the codes' padding holds does
     not matter."""
+
+    __slots__ = ("codes", "scale", "k")
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, k: int, group: int = GROUP):
         k, group = int(k), int(group)
@@ -40,16 +42,17 @@ class Q4Table:
         if codes.dim() != 2 or codes.shape[1] != groups * 16:
             raise ValueError(f"Q4Table: codes must be [n, {groups * 16}] for {k} columns, got "
                              f"{tuple(codes.shape)}")
-        if tuple(scale.shape) != (codes.shape[0], -(-k // group)):
+        if scale.shape != (codes.shape[0], -(-k // group)):
             raise ValueError(f"Q4Table: scale must be [{codes.shape[0]}, {-(-k // group)}], got "
                              f"{tuple(scale.shape)}")
         if codes.device != scale.device:
             raise ValueError(f"Q4Table: codes on {codes.device}, scale on {scale.device}")
         if group != GROUP:
             scale = scale.repeat_interleave(group // GROUP, dim=1)[:, :groups]
-        self.codes, self.scale, self.k = codes.contiguous(), scale.contiguous(), k
-        if self.codes.data_ptr() % 16:      # the kernels load 16 bytes
-            self.codes = self.codes.clone()
+        codes = codes.contiguous()
+        if codes.data_ptr() % 16:           # the kernels load 16 bytes
+            codes = codes.clone()
+        self.codes, self.scale, self.k = codes, scale.contiguous(), k
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -103,25 +106,28 @@ def q4_matmul(x: torch.Tensor, table: Q4Table,
     fp32 / bf16 / fp16 rows of any stride, at most 65535 of them."""
     if not isinstance(table, Q4Table):
         raise TypeError(f"q4_matmul: expected a Q4Table, got {type(table).__name__}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
+    codes, k = table.codes, table.k
+    if out_dtype is None:
+        out_dtype = x.dtype
     if out_dtype not in _lib.DTYPES:
         raise TypeError(f"q4_matmul: out_dtype must be float32, bfloat16 or float16, got "
                         f"{out_dtype}")
-    if x.dim() not in (1, 2) or x.shape[-1] != table.k:
-        raise ValueError(f"q4_matmul: x is {tuple(x.shape)}, the table has {table.k} columns")
-    if x.device != table.device:
-        raise ValueError(f"q4_matmul: x on {x.device}, table on {table.device}")
-    x2 = rows_of(x.detach(), "q4_matmul")
-    m, n = x2.shape[0], table.shape[0]
+    if x.dim() not in (1, 2) or x.shape[-1] != k:
+        raise ValueError(f"q4_matmul: x is {tuple(x.shape)}, the table has {k} columns")
+    device = x.device
+    if device != codes.device:
+        raise ValueError(f"q4_matmul: x on {device}, table on {codes.device}")
+    x2 = rows_of(x, "q4_matmul")
+    m, n = x2.shape[0], codes.shape[0]
     if m > 65535:
         raise NotImplementedError(f"q4_matmul: {m} rows of x, at most 65535")
-    out = torch.empty((m, n) if x.dim() == 2 else (n,), dtype=out_dtype, device=x.device)
+    out = torch.empty((m, n) if x.dim() == 2 else (n,), dtype=out_dtype, device=device)
     t = _lib.DTYPES[x.dtype]
     work = None
-    if table.k > SHORT_COLUMNS:
-        nbytes = _lib.lib().gnnrec_q4_matmul_work_bytes(t, m, table.k)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    launch("gnnrec_q4_matmul", x.device, t, _lib.DTYPES[out_dtype], m, x2.data_ptr(),
-           x2.stride(0), n, table.k, table.codes.data_ptr(), table.scale.data_ptr(),
-           out.data_ptr(), n, ptr(work))
+    if k > SHORT_COLUMNS:
+        nbytes = _lib.lib().gnnrec_q4_matmul_work_bytes(t, m, n, k)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    launch("gnnrec_q4_matmul", device, t, _lib.DTYPES[out_dtype], m, x2.data_ptr(),
+           x2.stride(0), n, k, codes.data_ptr(), table.scale.data_ptr(), out.data_ptr(), n,
+           ptr(work))
     return out

@@ -151,12 +151,15 @@ def test_c_entries_refuse_before_they_launch():
                      (dict(k=2 ** 30), "size"), (dict(codes=None), "null"),
                      (dict(codes=a + 4), "aligned"), (dict(x=None), "null"),
                      (dict(o=None), "null"), (dict(n=2 ** 50), "large"),
-                     (dict(k=257), "workspace"), (dict(k=257, work=a + 4), "workspace")):
+                     (dict(m=5, k=257), "workspace"),
+                     (dict(m=5, k=257, work=a + 4), "workspace")):
         rc, msg = q4(**kw)
         assert rc == -1 and word in msg, (kw, msg)
     assert q4(n=0)[0] == 0 and q4(m=0)[0] == 0
-    assert [L.gnnrec_q4_matmul_work_bytes(t, 5, k) for t in (0, 1, 2) for k in (256, 257)] \
-        == [0, 3 * 5 * 288 * 2, 0, 0, 0, 2 * 5 * 288 * 2]
+    work = L.gnnrec_q4_matmul_work_bytes
+    assert [work(t, 5, 4, k) for t in (0, 1, 2) for k in (256, 257)] \
+        == [0, 3 * 5 * 288 * 2, 0, 5 * 288 * 2, 0, 2 * 5 * 288 * 2]
+    assert work(1, 5, 4, 512) == 0 and work(0, 4, 4, 257) == 0 and work(9, 5, 4, 257) == 0
     assert L.gnnrec_quantize_q4(0, 4, 64, None, 64, a, a, None) == -1
     assert L.gnnrec_quantize_q4(9, 4, 64, a, 64, a, a, None) == -1
     assert L.gnnrec_dequantize_q4(4, 64, a, a, None, 64, None) == -1
