@@ -42,7 +42,7 @@ __global__ __launch_bounds__(kQ4Block) void quantize_q4_kernel(int64_t n, int64_
   if (row >= n) return;  // four threads of a group leave together
   const int64_t c = (int64_t)part * 8;
   float v[8];
-  load8(w + row * ldw + c, k - c, v);
+  load8(w + row * ldw, c, k, v);
   uint32_t top = 0;  // the magnitudes' bit patterns sort as the magnitudes, NaN above infinity
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(kQ4Block) void dequantize_q4_kernel(int64_t n, int6
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = e2m1(word >> (4 * e)) * s;
-  store8(out + row * ldo + c, k - c, v);
+  store8(out + row * ldo, c, k, v);
 }
 
 // ---- products -----------------------------------------------------------------------------
@@ -102,8 +102,6 @@ __global__ __launch_bounds__(kQ4Block) void dequantize_q4_kernel(int64_t n, int6
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <class T>
 struct Parts;
@@ -344,7 +342,7 @@ __global__ __launch_bounds__(kQ4Block, FEW ? 4 : 3) void q4_walk_kernel(const T*
   for (int i = threadIdx.x; i < users * per; i += kQ4Block) {
     const int u = i / per, c = i - u * per;
     float v[8];
-    load8(x + (user0 + u) * ldx + c * 8, p.k - c * 8, v);
+    load8(x + (user0 + u) * ldx, c * 8, p.k, v);
     u32x4 parts[kP];
     split8(v, parts);
 #pragma unroll
@@ -419,7 +417,7 @@ __global__ __launch_bounds__(WK * 64, 4) void q4_few_kernel(const T* __restrict_
   for (int u = 0; u < users; ++u)
     for (int c = threadIdx.x; c < per; c += WK * 64) {
       float v[8];
-      load8(x + (user0 + u) * ldx + c * 8, p.k - c * 8, v);
+      load8(x + (user0 + u) * ldx, c * 8, p.k, v);
       u32x4 parts[kP];
       split8(v, parts);
 #pragma unroll
@@ -516,7 +514,7 @@ __global__ __launch_bounds__(kQ4Block) void split_users_kernel(const T* __restri
   const int64_t per = kp / 8, row = i / per, c = (i - row * per) * 8;
   if (row >= m) return;
   float v[8];
-  load8(x + row * ldx + c, k - c, v);
+  load8(x + row * ldx, c, k, v);
   u32x4 w[kP];
   split8(v, w);
 #pragma unroll

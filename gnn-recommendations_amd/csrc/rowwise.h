@@ -20,28 +20,74 @@ inline int with_dtype(int32_t t, F&& f) {
 }
 inline bool dtype_ok(int32_t t) { return t == GNNREC_F32 || t == GNNREC_BF16 || t == GNNREC_F16; }
 
-// Eight neighbouring elements; aligned as one element only, so that rows of any width and
-// stride load with 16-B instructions (the hardware takes unaligned vector accesses).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Eight neighbouring elements as they lie in memory. Aligned as one element only, so that rows of
+// any width and stride load with 16-B instructions (the hardware takes unaligned vectors).
 template <class T>
 struct __attribute__((packed)) Eight {
   T v[8];
 };
-
-// v[e] = p[e] for e < n, 0 for the others. n >= 8: one vector access.
 template <class T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int64_t n, float (&v)[8]) {
-  if (n >= 8) {
-    const Eight<T> t = *reinterpret_cast<const Eight<T>*>(p);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)t.v[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.f;
+struct Raw {
+  uint32_t w[2 * sizeof(T)];
+};
+
+// Columns c .. c + 7 of a row of d values, 0 behind its end (also for a c behind it): fetch8 is
+// the memory access alone, so that several are in flight, and take8 what follows it. No lane
+// branches: a row's last, partial eight is read from the row's last eight values and shifted down,
+// since a lane that loaded its few values one by one would hold up the wave for as many round
+// trips. NARROW: d < 8, the row's values one by one.
+template <class T, bool NARROW>
+__device__ __forceinline__ Raw<T> fetch8(const T* __restrict__ row, int64_t c, int64_t d) {
+  if (!NARROW) {
+    const int64_t at = c < d - 8 ? c : d - 8;
+    return __builtin_bit_cast(Raw<T>, *reinterpret_cast<const Eight<T>*>(row + at));
   }
+  Eight<T> e;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e.v[i] = row[i < d ? i : d - 1];
+  return __builtin_bit_cast(Raw<T>, e);
+}
+
+template <class T, bool NARROW>
+__device__ __forceinline__ void take8(Raw<T> t, int64_t c, int64_t d, float (&v)[8]) {
+  constexpr int kWords = 2 * sizeof(T), kPer = 4 / sizeof(T);  // elements a word
+  if (!NARROW && (d & 7)) {
+    const int s = c > d - 8 ? (int)(c - d) & 7 : 0;
+#pragma unroll
+    for (int bit = 4; bit >= 1; bit >>= 1) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        uint32_t from;
+        if (bit >= kPer) {
+          from = i + bit / kPer < kWords ? t.w[i + bit / kPer] : 0u;
+        } else {  // half a word
+          from = (t.w[i] >> 16) | (i + 1 < kWords ? t.w[i + 1] << 16 : 0u);
+        }
+        t.w[i] = s & bit ? from : t.w[i];
+      }
+    }
+  }
+  const Eight<T> e = __builtin_bit_cast(Eight<T>, t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (NARROW ? c == 0 && i < d : c < d) ? (float)e.v[i] : 0.f;
+}
+
+// Both at once, for any width.
+template <class T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c, int64_t d,
+                                      float (&v)[8]) {
+  if (d >= 8) take8<T, false>(fetch8<T, false>(row, c, d), c, d, v);
+  else take8<T, true>(fetch8<T, true>(row, c, d), c, d, v);
 }
 
 template <class T>
-__device__ __forceinline__ void store8(T* __restrict__ p, int64_t n, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* __restrict__ row, int64_t c, int64_t d,
+                                       const float (&v)[8]) {
+  T* p = row + c;
+  const int64_t n = d - c;
   if (n >= 8) {
     Eight<T> t;
 #pragma unroll
