@@ -3,7 +3,7 @@ scripts/run_all_experiments.py), kept to the plumbing the propagation path needs
 
     python run_all.py [--quick] [--skip-check] [--models lightgcn ...] [--datasets ml-100k]
                       [--seeds 42 43] [--n_layers K] [--embedding_dim d] [--epochs E]
-                      [--device cpu|cuda]
+                      [--device cpu|cuda] [--item_bits 4|32]
 
 For every dataset x model x seed: load the dataset (data/processed/<name> if present, else
 data/raw/<name>/u.data or ratings.dat through the reference's preprocessing, else an
@@ -106,6 +106,8 @@ def main(argv=None) -> int:
     ap.add_argument("--embedding_dim", type=int, default=None)
     ap.add_argument("--epochs", type=int, default=None)
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
+    ap.add_argument("--item_bits", type=int, default=32, choices=[4, 32],
+                    help="4: rank against the item table in 4 bits (needs a ROCm device)")
     ap.add_argument("--output", default=str(ROOT / "results" / "run_all.json"))
     a = ap.parse_args(argv)
     if a.quick:
@@ -129,7 +131,8 @@ def main(argv=None) -> int:
                     adj = ds.get_graph(device) if device.type == "cuda" else ds.get_torch_adjacency()
                     rec["training_time"] = train_bpr(model, ds, adj, cfg, epochs, device, seed)
                     t0 = time.time()
-                    rec["test_metrics"] = Evaluator(device=device).evaluate(model, ds, adj_matrix=adj)
+                    rec["test_metrics"] = Evaluator(
+                        device=device, item_bits=a.item_bits).evaluate(model, ds, adj_matrix=adj)
                     rec["eval_time"] = time.time() - t0
                     rec.update(status="success", n_users=ds.n_users, n_items=ds.n_items,
                                n_train=len(ds.train_data), epochs=epochs)

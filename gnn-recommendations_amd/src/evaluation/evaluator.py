@@ -13,7 +13,7 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 
-from ..ops import CsrGraph, score_topk, uses_native
+from ..ops import CsrGraph, q4_matmul, quantize_q4, score_topk, uses_native
 
 
 def compute_metrics_from_topk(topk_items, user_ids: List[int], ground_truth: Dict[int, List[int]],
@@ -133,16 +133,27 @@ def embedding_statistics(emb, exact_limit: int = 65536, chunk: int = 4096,
 
 
 class Evaluator:
-    def __init__(self, k_values=(10, 20), device: Optional[torch.device] = None):
+    """item_bits = 4 ranks against the item table in 4 bits (ops.quantize_q4), as a server that
+    holds it so would answer: the metrics then tell what that table costs in quality. The same
+    order and masking; needs a ROCm device."""
+
+    def __init__(self, k_values=(10, 20), device: Optional[torch.device] = None,
+                 item_bits: int = 32):
         self.k_values = list(k_values)
         self.device = device or torch.device("cuda" if torch.cuda.is_available() else "cpu")
+        if item_bits not in (4, 32):
+            raise ValueError(f"Evaluator: item_bits must be 4 or 32, got {item_bits}")
+        if item_bits == 4 and torch.device(self.device).type != "cuda":
+            raise ValueError("Evaluator: 4-bit items need a ROCm device")
+        self.item_bits = item_bits
 
     def topk(self, user_emb, item_emb, users, k, seen_ptr, seen_col, batch_size=None):
         """[len(users), k] int64 top-k item ids (fixed tie order). On the GPU nothing of size
         batch x n_items is materialised, so the batch is large (16384 users) and the kernel's
         item split fills the chip; the CPU path keeps the reference's 2048."""
-        if batch_size is None:
-            batch_size = 16384 if user_emb.is_cuda else 2048
+        table = quantize_q4(item_emb) if self.item_bits == 4 else None
+        if batch_size is None:   # (4-bit items: the batch's scores are materialised)
+            batch_size = 64 if table is not None else 16384 if user_emb.is_cuda else 2048
         rows = []
         for s in range(0, len(users), batch_size):
             b = torch.as_tensor(users[s:s + batch_size], dtype=torch.long, device=user_emb.device)
@@ -152,13 +163,19 @@ class Evaluator:
             # gather the batch's seen lists without a per-user loop
             src = np.repeat(bp - sub_ptr[:-1], counts) + np.arange(int(sub_ptr[-1]))
             sub_col = seen_col[src] if src.size else np.zeros(0, np.int32)
-            if user_emb.is_cuda:
+            if table is None and user_emb.is_cuda:
                 idx, _ = score_topk(user_emb[b], item_emb, k, torch.from_numpy(sub_ptr),
                                     torch.from_numpy(sub_col.astype(np.int32)))
             else:
-                sc = user_emb[b] @ item_emb.T
-                for r in range(len(b)):
-                    sc[r, torch.from_numpy(sub_col[sub_ptr[r]:sub_ptr[r + 1]].astype(np.int64))] = float("-inf")
+                if table is not None:
+                    sc = q4_matmul(user_emb[b], table, out_dtype=torch.float32)
+                    at = np.repeat(np.arange(len(b)), counts)
+                    sc[torch.from_numpy(at).to(sc.device),
+                       torch.from_numpy(sub_col.astype(np.int64)).to(sc.device)] = float("-inf")
+                else:
+                    sc = user_emb[b] @ item_emb.T
+                    for r in range(len(b)):
+                        sc[r, torch.from_numpy(sub_col[sub_ptr[r]:sub_ptr[r + 1]].astype(np.int64))] = float("-inf")
                 order = torch.sort(sc, dim=1, descending=True, stable=True).indices
                 idx = order[:, :k]
             rows.append(idx.cpu())

@@ -516,7 +516,12 @@ def ngcf_forward_dist(dg: DistributedGraph, model, x0_pad: torch.Tensor, *,
     x_in = x0_pad
     for k, (layer, gs) in enumerate(zip(model.layers, gs_layers)):
         y = local[:, c0:c0 + widths[k + 1]]
-        layer_fn(dg.shard, x_in, x_local, layer, gs, y)
+        if layer.norm is None:
+            layer_fn(dg.shard, x_in, x_local, layer, gs, y)
+        else:    # the norm is row-local, between the layer and its Group-and-Shuffle transform
+            layer_fn(dg.shard, x_in, x_local, layer, None, y)
+            out = layer.normalised(y, x_local)
+            y.copy_(gs(out) if gs is not None else out)
         x_local = y
         c0 += widths[k + 1]
         if k + 1 < len(model.layers):
