@@ -14,7 +14,7 @@ namespace gnnrec {
 
 constexpr int kDropBlock = 256;
 
-template <class T, bool BWD, bool NARROW>
+template <class T, bool BWD, Edge EDGE>
 __global__ __launch_bounds__(kDropBlock) void dropout_kernel(
     int64_t rows, int64_t d, int64_t nb, const T* __restrict__ x, int64_t ldx,
     const T* __restrict__ dy, int64_t lddy, T* __restrict__ out, int64_t ldo, Drop drop) {
@@ -28,30 +28,31 @@ __global__ __launch_bounds__(kDropBlock) void dropout_kernel(
   const int64_t c = (int64_t)cb * 8;
   float f[8], v[8];
   if (!BWD) {
-    const Raw<T> rx = fetch8<T, NARROW>(x + row * ldx, c, d);
+    const Raw<T> rx = fetch8<T, EDGE>(x + row * ldx, c, d);
     drop_factors(drop, drop_key(drop), row, cb, f);  // while the values are on their way
-    take8<T, NARROW>(rx, c, d, v);
+    take8<T, EDGE>(rx, c, d, v);
+    if (drop.slope != 1.f) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = v[e] > 0.f ? v[e] : v[e] * drop.slope;
-      v[e] = f[e] != 0.f ? a * f[e] : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = v[e] > 0.f ? v[e] : v[e] * drop.slope;
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = masked(v[e], f[e]);
   } else {
-    const Raw<T> rdy = fetch8<T, NARROW>(dy + row * lddy, c, d);
+    const Raw<T> rdy = fetch8<T, EDGE>(dy + row * lddy, c, d);
     Raw<T> rx;
-    if (drop.slope != 1.f) rx = fetch8<T, NARROW>(x + row * ldx, c, d);
+    if (drop.slope != 1.f) rx = fetch8<T, EDGE>(x + row * ldx, c, d);
     drop_factors(drop, drop_key(drop), row, cb, f);
-    take8<T, NARROW>(rdy, c, d, v);
+    take8<T, EDGE>(rdy, c, d, v);
     if (drop.slope != 1.f) {
       float xv[8];
-      take8<T, NARROW>(rx, c, d, xv);
+      take8<T, EDGE>(rx, c, d, xv);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = xv[e] > 0.f ? v[e] : v[e] * drop.slope;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = f[e] != 0.f ? v[e] * f[e] : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = masked(v[e], f[e]);
   }
-  store8(out + row * ldo, c, d, v);
+  store8<T, EDGE>(out + row * ldo, c, d, v);
 }
 
 template <bool BWD>
@@ -71,7 +72,9 @@ static int run_dropout(const char* what, int32_t dtype, int64_t rows, int64_t d,
   GNNREC_REQUIRE(blocks <= 0x7fffffff, "%s: table too large", what);
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    auto* kernel = d < 8 ? dropout_kernel<T, BWD, true> : dropout_kernel<T, BWD, false>;
+    auto* kernel = d < 8        ? dropout_kernel<T, BWD, kNarrow>
+                   : d % 8 == 0 ? dropout_kernel<T, BWD, kFull>
+                                : dropout_kernel<T, BWD, kRagged>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kDropBlock), 0, as_hip(stream), rows,
                        d, nb, (const T*)x, ldx, (const T*)dy, lddy, (T*)out, ldo, drop);
     return check_launch(what);

@@ -36,17 +36,17 @@ struct NormIn {
   Drop drop;
 };
 
-// Eight values of w or b (`fill` where there is none).
-template <class T, bool NARROW>
+// Eight values of w or b (`fill` where there is none; anything behind the row's end).
+template <class T, Edge EDGE>
 __device__ __forceinline__ void load_param(const void* p, int32_t f32, int64_t c, int64_t d,
                                            float fill, float (&v)[8]) {
   if (!p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = fill;
   } else if (f32) {
-    take8<float, NARROW>(fetch8<float, NARROW>((const float*)p, c, d), c, d, v);
+    take8<float, EDGE, false>(fetch8<float, EDGE>((const float*)p, c, d), c, d, v);
   } else {
-    take8<T, NARROW>(fetch8<T, NARROW>((const T*)p, c, d), c, d, v);
+    take8<T, EDGE, false>(fetch8<T, EDGE>((const T*)p, c, d), c, d, v);
   }
 }
 
@@ -56,32 +56,35 @@ __device__ __forceinline__ float moved(float v) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
 
-// The sum over aligned groups of L lanes, in every lane of them: pairs and quads, then mirrors
-// (a group's halves hold equal values), then the lane rows through permlane swaps.
+// The sums of a and b over aligned groups of L lanes, in every lane of them: pairs and quads, then
+// mirrors (a group's halves hold equal values), then the lane rows through permlane swaps.
 template <int L>
-__device__ __forceinline__ float lane_sum(float v) {
-  v += moved<0xB1>(v);                // quad_perm 1 0 3 2
-  v += moved<0x4E>(v);                // quad_perm 2 3 0 1
-  v += moved<0x141>(v);               // mirror within 8
-  if (L >= 16) v += moved<0x140>(v);  // mirror within 16
+__device__ __forceinline__ void lane_sum2(float& a, float& b) {
+  auto step = [&](float x, float y) { a += x, b += y; };
+  step(moved<0xB1>(a), moved<0xB1>(b));                // quad_perm 1 0 3 2
+  step(moved<0x4E>(a), moved<0x4E>(b));                // quad_perm 2 3 0 1
+  step(moved<0x141>(a), moved<0x141>(b));              // mirror within 8
+  if (L >= 16) step(moved<0x140>(a), moved<0x140>(b));  // mirror within 16
   if (L >= 32) {
-    const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v),
-                                                     false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    const u32x2 ra = __builtin_amdgcn_permlane16_swap(ua, ua, false, false);
+    const u32x2 rb = __builtin_amdgcn_permlane16_swap(ub, ub, false, false);
+    a = __uint_as_float(ra[0]) + __uint_as_float(ra[1]);
+    b = __uint_as_float(rb[0]) + __uint_as_float(rb[1]);
   }
   if (L >= 64) {
-    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
-                                                     false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    const u32x2 ra = __builtin_amdgcn_permlane32_swap(ua, ua, false, false);
+    const u32x2 rb = __builtin_amdgcn_permlane32_swap(ub, ub, false, false);
+    a = __uint_as_float(ra[0]) + __uint_as_float(ra[1]);
+    b = __uint_as_float(rb[0]) + __uint_as_float(rb[1]);
   }
-  return v;
 }
 
 // Sums a and b over the TPR lanes (or waves) that share a row.
 template <int TPR>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
-  a = lane_sum<TPR < 64 ? TPR : 64>(a);
-  b = lane_sum<TPR < 64 ? TPR : 64>(b);
+  lane_sum2<TPR < 64 ? TPR : 64>(a, b);
   if (TPR > 64) {  // the workgroup is one row: every thread adds the waves' sums in one order
     constexpr int kWaves = TPR / 64;
     const int w = threadIdx.x >> 6;
@@ -101,7 +104,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
 }
 
 // A row's inputs on their way: this lane's NV blocks of each table.
-template <class T, int TPR, int NV, bool NARROW, int TABLES>
+template <class T, int TPR, int NV, Edge EDGE, int TABLES>
 struct RowIn {
   Raw<T> raw[TABLES][NV];
 
@@ -110,10 +113,11 @@ struct RowIn {
     if (!p) return;
 #pragma unroll
     for (int j = from; j < to; ++j)
-      raw[k][j] = fetch8<T, NARROW>((const T*)p + row * ld, (int64_t)(j * TPR + t) * 8, d);
+      raw[k][j] = fetch8<T, EDGE>((const T*)p + row * ld, (int64_t)(j * TPR + t) * 8, d);
   }
+  template <bool ZERO>
   __device__ __forceinline__ void take(int k, int j, int64_t d, int t, float (&v)[8]) const {
-    take8<T, NARROW>(raw[k][j], (int64_t)(j * TPR + t) * 8, d, v);
+    take8<T, EDGE, ZERO>(raw[k][j], (int64_t)(j * TPR + t) * 8, d, v);
   }
 };
 
@@ -138,48 +142,53 @@ __device__ __forceinline__ void activate(const NormIn& in, uint64_t key, int64_t
     drop_factors(in.drop, key, row, cb, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      h[e] = f[e] != 0.f ? h[e] * f[e] : 0.f;
+      h[e] = masked(h[e], f[e]);
       if (FACTORS) fx[e] *= f[e];
     }
   }
 }
 
-// h of one row from x (table 0) and the residual (table 1), and with FACTORS dx / dh.
-template <class T, int TPR, int NV, bool NARROW, bool FACTORS, class In>
+// h of one row from x (table 0) and the residual (table 1), and with FACTORS dx / dh. PLAIN: h is
+// x. What a lane holds behind the row's end is anything.
+template <bool PLAIN, bool FACTORS, int TPR, int NV, class In>
 __device__ __forceinline__ void form_h(const NormIn& in, uint64_t key, const In& raw, int64_t row,
                                        int t, float (&h)[NV][8], float (&fx)[NV][8]) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    raw.take(0, j, in.d, t, h[j]);
+    raw.template take<false>(0, j, in.d, t, h[j]);
+    if (PLAIN) continue;
     activate<FACTORS>(in, key, row, (uint32_t)(j * TPR + t), h[j], fx[j]);
     if (in.res) {
       float r[8];
-      raw.take(1, j, in.d, t, r);
+      raw.template take<false>(1, j, in.d, t, r);
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[j][e] += r[e];
     }
   }
 }
 
-// h -> u in place (columns behind the row's end: 0); returns r.
-template <int TPR, int NV>
+// h -> u in place; returns r. Behind the row's end u is finite where the row is (the gradients
+// there are 0, and nothing of it is stored).
+template <int TPR, int NV, Edge EDGE>
 __device__ __forceinline__ float normalize(const NormIn& in, int t, float (&h)[NV][8],
                                            float* red) {
   const float inv = 1.f / (float)in.d;
   float s = 0.f, unused = 0.f;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    const int n = (int)in.d - (j * TPR + t) * 8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += h[j][e];
+    for (int e = 0; e < 8; ++e) s += EDGE == kFull || e < n ? h[j][e] : 0.f;
+  }
   row_sum2<TPR>(s, unused, red);
   const float mean = s * inv;
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int64_t n = in.d - (int64_t)(j * TPR + t) * 8;
+    const int n = (int)in.d - (j * TPR + t) * 8;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      h[j][e] = e < n ? h[j][e] - mean : 0.f;
+      h[j][e] = EDGE == kFull || e < n ? h[j][e] - mean : 0.f;
       s1 += h[j][e];
       s2 = fmaf(h[j][e], h[j][e], s2);
     }
@@ -189,15 +198,13 @@ __device__ __forceinline__ float normalize(const NormIn& in, int t, float (&h)[N
   const float var = fmaxf(fmaf(-off, off, s2 * inv), 0.f);
   const float r = 1.f / __builtin_sqrtf(var + in.eps);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int64_t n = in.d - (int64_t)(j * TPR + t) * 8;
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[j][e] = e < n ? (h[j][e] - off) * r : 0.f;
-  }
+    for (int e = 0; e < 8; ++e) h[j][e] = (h[j][e] - off) * r;
   return r;
 }
 
-template <class T, int TPR, int NV, bool NARROW>
+template <class T, int TPR, int NV, Edge EDGE, bool PLAIN>
 __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock) void norm_forward_kernel(
     NormIn in, T* __restrict__ y, int64_t ldy, T* __restrict__ hout, int64_t ldh) {
   constexpr int kBlock = TPR > kNormBlock ? TPR : kNormBlock;
@@ -205,28 +212,29 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock) void norm_forw
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * (kBlock / TPR) + threadIdx.x / TPR;
   if (row >= in.rows) return;  // whole rows only: the lanes of a row leave together
-  RowIn<T, TPR, NV, NARROW, 2> raw;
+  RowIn<T, TPR, NV, EDGE, PLAIN ? 1 : 2> raw;
   raw.fetch(0, in.x, in.ldx, row, in.d, t);
-  raw.fetch(1, in.res, in.ldr, row, in.d, t);
+  if (!PLAIN) raw.fetch(PLAIN ? 0 : 1, in.res, in.ldr, row, in.d, t);
   float h[NV][8], none[NV][8];
-  form_h<T, TPR, NV, NARROW, false>(in, in.dropping ? drop_key(in.drop) : 0, raw, row, t, h, none);
+  form_h<PLAIN, false, TPR, NV>(in, in.dropping ? drop_key(in.drop) : 0, raw, row, t, h,
+                                none);
   if (hout) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t c = (int64_t)(j * TPR + t) * 8;
-      store8(hout + row * ldh, c, in.d, h[j]);
+      store8<T, EDGE>(hout + row * ldh, c, in.d, h[j]);
     }
   }
-  normalize<TPR, NV>(in, t, h, red);
+  normalize<TPR, NV, EDGE>(in, t, h, red);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int64_t c = (int64_t)(j * TPR + t) * 8;
     float w[8], b[8];
-    load_param<T, NARROW>(in.w, in.w_f32, c, in.d, 1.f, w);
-    load_param<T, NARROW>(in.b, in.w_f32, c, in.d, 0.f, b);
+    load_param<T, EDGE>(in.w, in.w_f32, c, in.d, 1.f, w);
+    load_param<T, EDGE>(in.b, in.w_f32, c, in.d, 0.f, b);
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[j][e] = fmaf(h[j][e], w[e], b[e]);
-    store8(y + row * ldy, c, in.d, h[j]);
+    store8<T, EDGE>(y + row * ldy, c, in.d, h[j]);
   }
 }
 
@@ -236,7 +244,7 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock) void norm_forw
 // us for fewer registers). With 1024 lanes, of 128 registers each, so is x again with its mask, and
 // dw and db are summed in LDS (LATE: in registers they spilled: 5003 x 16384 bf16 743 us, in LDS
 // 311).
-template <class T, int TPR, int NV, bool NARROW>
+template <class T, int TPR, int NV, Edge EDGE, bool PLAIN>
 __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
                              NV == 1 && TPR <= 64 ? 4 : 1) void norm_backward_kernel(
     NormIn in, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ dh, int64_t lddh,
@@ -261,13 +269,14 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
 #pragma unroll
       for (int e = 0; e < 8; ++e) own[k * TPR * 8 + e] = 0.f;
   }
-  using In = RowIn<T, TPR, NV, NARROW, 4>;
+  constexpr int kDy = PLAIN ? 1 : 2, kDh = PLAIN ? 1 : 3;  // their places among the tables
+  using In = RowIn<T, TPR, NV, EDGE, PLAIN ? 2 : 4>;
   auto fetch = [&](In& raw, int64_t row) {
     raw.fetch(0, in.x, in.ldx, row, in.d, t);
-    raw.fetch(1, in.res, in.ldr, row, in.d, t);
+    if (!PLAIN) raw.fetch(1, in.res, in.ldr, row, in.d, t);
     if (!kWhenNeeded) {
-      raw.fetch(2, dy, lddy, row, in.d, t);
-      raw.fetch(3, dh, lddh, row, in.d, t);
+      raw.fetch(kDy, dy, lddy, row, in.d, t);
+      if (!PLAIN) raw.fetch(kDh, dh, lddh, row, in.d, t);
     }
   };
   In next;
@@ -282,15 +291,15 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
       fetch(raw, row);
     }
     float u[NV][8], fx[NV][8], g[NV][8];
-    form_h<T, TPR, NV, NARROW, !LATE>(in, key, raw, row, t, u, fx);
-    const float r = normalize<TPR, NV>(in, t, u, red);
+    form_h<PLAIN, !LATE, TPR, NV>(in, key, raw, row, t, u, fx);
+    const float r = normalize<TPR, NV, EDGE>(in, t, u, red);
     float s1 = 0.f, s2 = 0.f;
-    if (kWhenNeeded) raw.fetch(2, dy, lddy, row, in.d, t);
+    if (kWhenNeeded) raw.fetch(kDy, dy, lddy, row, in.d, t);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float w[8];
-      raw.take(2, j, in.d, t, g[j]);
-      load_param<T, NARROW>(in.w, in.w_f32, (int64_t)(j * TPR + t) * 8, in.d, 1.f, w);
+      raw.template take<true>(kDy, j, in.d, t, g[j]);
+      load_param<T, EDGE>(in.w, in.w_f32, (int64_t)(j * TPR + t) * 8, in.d, 1.f, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (LATE) {
@@ -309,29 +318,31 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
     row_sum2<TPR>(s1, s2, red);
     s1 *= inv;
     s2 *= inv;
-    if (kWhenNeeded) raw.fetch(3, dh, lddh, row, in.d, t);
+    if (kWhenNeeded && !PLAIN) raw.fetch(kDh, dh, lddh, row, in.d, t);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t c = (int64_t)(j * TPR + t) * 8;
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[j][e] = r * (g[j][e] - fmaf(u[j][e], s2, s1));
-      if (dh) {
+      if (!PLAIN && dh) {
         float v[8];
-        raw.take(3, j, in.d, t, v);
+        raw.template take<false>(kDh, j, in.d, t, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[j][e] += v[e];
       }
-      if (dres) store8(dres + row * lddr, c, in.d, g[j]);
+      if (!PLAIN && dres) store8<T, EDGE>(dres + row * lddr, c, in.d, g[j]);
       if (dx) {
-        if (LATE) {
+        if (LATE && !PLAIN) {
           raw.fetch(0, in.x, in.ldx, row, in.d, t, j, j + 1);
           float a[8];
-          raw.take(0, j, in.d, t, a);
+          raw.template take<false>(0, j, in.d, t, a);
           activate<true>(in, key, row, (uint32_t)(j * TPR + t), a, fx[j]);
         }
+        if (!PLAIN) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[j][e] = fx[j][e] != 0.f ? g[j][e] * fx[j][e] : 0.f;
-        store8(dx + row * lddx, c, in.d, g[j]);
+          for (int e = 0; e < 8; ++e) g[j][e] = masked(g[j][e], fx[j][e]);
+        }
+        store8<T, EDGE>(dx + row * lddx, c, in.d, g[j]);
       }
     }
   }
@@ -391,23 +402,37 @@ __global__ __launch_bounds__(kSumCols* kSumSlices) void norm_sum_kernel(
 }
 
 // Lanes a row and blocks a lane by the row's width (blocks of eight columns): one wave holds up
-// to 1024 columns, wider rows take a workgroup.
+// to 1024 columns, wider rows take a workgroup. Narrow shapes have an instance for rows that fill
+// every lane (64, 128, 256, 512, 1024 columns: no masks), wide ones for the norm alone (no
+// registers for a residual and a mask).
+template <int TPR, int NV, Edge EDGE, bool PLAIN>
+struct Shape {
+  static constexpr int tpr = TPR, nv = NV;
+  static constexpr Edge edge = EDGE;
+  static constexpr bool plain = PLAIN;
+};
+template <int TPR, int NV, class F>
+static int one_wave(int64_t d, F&& f) {
+  return d == TPR * NV * 8 ? f(Shape<TPR, NV, kFull, false>{})
+                           : f(Shape<TPR, NV, kRagged, false>{});
+}
+template <int TPR, int NV, class F>
+static int workgroup(bool plain, F&& f) {
+  return plain ? f(Shape<TPR, NV, kRagged, true>{}) : f(Shape<TPR, NV, kRagged, false>{});
+}
 template <class F>
-static int with_shape(int64_t d, F&& f) {
+static int with_shape(int64_t d, bool plain, F&& f) {
   const int64_t nb = ceil_div(d, 8);
-  const std::integral_constant<int, 1> i1{};
-  const std::integral_constant<int, 2> i2{};
-  const std::false_type wide{};
-  if (d < 8) return f(std::integral_constant<int, 8>{}, i1, std::true_type{});
-  if (nb <= 8) return f(std::integral_constant<int, 8>{}, i1, wide);
-  if (nb <= 16) return f(std::integral_constant<int, 16>{}, i1, wide);
-  if (nb <= 32) return f(std::integral_constant<int, 32>{}, i1, wide);
-  if (nb <= 64) return f(std::integral_constant<int, 64>{}, i1, wide);
-  if (nb <= 128) return f(std::integral_constant<int, 64>{}, i2, wide);
-  if (nb <= 256) return f(std::integral_constant<int, 256>{}, i1, wide);
-  if (nb <= 512) return f(std::integral_constant<int, 256>{}, i2, wide);
-  if (nb <= 1024) return f(std::integral_constant<int, 512>{}, i2, wide);
-  return f(std::integral_constant<int, 1024>{}, i2, wide);
+  if (d < 8) return f(Shape<8, 1, kNarrow, false>{});
+  if (nb <= 8) return one_wave<8, 1>(d, f);
+  if (nb <= 16) return one_wave<16, 1>(d, f);
+  if (nb <= 32) return one_wave<32, 1>(d, f);
+  if (nb <= 64) return one_wave<64, 1>(d, f);
+  if (nb <= 128) return one_wave<64, 2>(d, f);
+  if (nb <= 256) return workgroup<256, 1>(plain, f);
+  if (nb <= 512) return workgroup<256, 2>(plain, f);
+  if (nb <= 1024) return workgroup<512, 2>(plain, f);
+  return workgroup<1024, 2>(plain, f);
 }
 
 // Rows a workgroup holds at a time, and workgroups of the backward pass: as many as are resident
@@ -415,8 +440,8 @@ static int with_shape(int64_t d, F&& f) {
 // passes: 512 workgroups 105 us, 1024 111, 256 126; 2M x 64 fp32 block: 1024 966, 1280 1361.
 static int64_t rows_per_block(int64_t d) {
   int64_t r = 1;
-  with_shape(d, [&](auto tpr, auto, auto) {
-    r = tpr.value < kNormBlock ? kNormBlock / tpr.value : 1;
+  with_shape(d, false, [&](auto s) {
+    r = s.tpr < kNormBlock ? kNormBlock / s.tpr : 1;
     return 0;
   });
   return r;
@@ -424,6 +449,10 @@ static int64_t rows_per_block(int64_t d) {
 static int64_t backward_blocks(int64_t rows, int64_t d) {
   const int64_t b = ceil_div(rows, rows_per_block(d)), most = d <= 1024 ? 1024 : 512;
   return b < most ? b : most;
+}
+
+static bool is_plain(const NormIn& in) {
+  return !in.res && !in.dropping && in.drop.slope == 1.f;
 }
 
 static int check_norm(NormIn* in, const char* what, int32_t dtype, int32_t wdtype, int64_t rows,
@@ -464,10 +493,11 @@ extern "C" int gnnrec_layer_norm_forward(int32_t dtype, int32_t wdtype, int64_t 
   GNNREC_REQUIRE(y, "layer_norm_forward: null pointer");
   return with_dtype(dtype, [&](auto e) {
     using T = decltype(e);
-    return with_shape(d, [&](auto tpr, auto nv, auto narrow) {
-      constexpr int kBlock = tpr.value > kNormBlock ? tpr.value : kNormBlock;
-      hipLaunchKernelGGL((norm_forward_kernel<T, tpr.value, nv.value, narrow.value>),
-                         dim3((unsigned)ceil_div(rows, kBlock / tpr.value)), dim3(kBlock), 0,
+    return with_shape(d, is_plain(in), [&](auto s) {
+      using S = decltype(s);
+      constexpr int kBlock = S::tpr > kNormBlock ? S::tpr : kNormBlock;
+      hipLaunchKernelGGL((norm_forward_kernel<T, S::tpr, S::nv, S::edge, S::plain>),
+                         dim3((unsigned)ceil_div(rows, kBlock / S::tpr)), dim3(kBlock), 0,
                          as_hip(stream), in, (T*)y, ldy, (T*)h, ldh);
       return check_launch("layer_norm_forward");
     });
@@ -497,9 +527,10 @@ extern "C" int gnnrec_layer_norm_backward(int32_t dtype, int32_t wdtype, int64_t
   if (rows > 0) {
     const int rc2 = with_dtype(dtype, [&](auto e) {
       using T = decltype(e);
-      return with_shape(d, [&](auto tpr, auto nv, auto narrow) {
-        constexpr int kBlock = tpr.value > kNormBlock ? tpr.value : kNormBlock;
-        hipLaunchKernelGGL((norm_backward_kernel<T, tpr.value, nv.value, narrow.value>),
+      return with_shape(d, is_plain(in) && !dh && !dres, [&](auto s) {
+        using S = decltype(s);
+        constexpr int kBlock = S::tpr > kNormBlock ? S::tpr : kNormBlock;
+        hipLaunchKernelGGL((norm_backward_kernel<T, S::tpr, S::nv, S::edge, S::plain>),
                            dim3((unsigned)blocks), dim3(kBlock), 0, as_hip(stream), in, (const T*)dy, lddy, (const T*)dh,
                            lddh, (T*)dx, lddx, (T*)dres, lddr, dw || db ? work : nullptr);
         return check_launch("layer_norm_backward");

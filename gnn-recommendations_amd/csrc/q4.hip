@@ -527,7 +527,7 @@ __global__ __launch_bounds__(kQ4Block) void split_users_kernel(const T* __restri
 constexpr int64_t kWalkGrid = 768, kWalkGridTiled = 384, kSplitGrid = 1024;
 // LDS that the users' fragments or rows may take: two workgroups still fit a CU (160 KB), and
 // with the joined sums the rows stay below 64 KB.
-constexpr int64_t kWalkBytes = 64 * 1024, kFewBytes = 48 * 1024;
+constexpr int64_t kWalkBytes = 64 * 1024, kFewBytes = 50 * 1024;
 // Items from which waves walk long rows alone (125 000 x 512, one user: 13.1 us, split 49.3), and
 // from which a tile set is four tiles (4 users x 30 000 x 1 000: one tile 10.7 us, four 14.9).
 constexpr int64_t kManyItems = 16384, kWideItems = 65536;

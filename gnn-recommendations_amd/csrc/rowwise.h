@@ -34,15 +34,20 @@ struct Raw {
   uint32_t w[2 * sizeof(T)];
 };
 
-// Columns c .. c + 7 of a row of d values, 0 behind its end (also for a c behind it): fetch8 is
-// the memory access alone, so that several are in flight, and take8 what follows it. No lane
-// branches: a row's last, partial eight is read from the row's last eight values and shifted down,
-// since a lane that loaded its few values one by one would hold up the wave for as many round
-// trips. NARROW: d < 8, the row's values one by one.
-template <class T, bool NARROW>
+// How the lanes' eights meet a row's end. kFull: every lane's eight columns lie in the row.
+// kRagged: the row's last eight may be partial and lanes may start behind its end. kNarrow: the
+// row has fewer than eight values.
+enum Edge { kFull, kRagged, kNarrow };
+
+// Columns c .. c + 7 of a row of d values, 0 behind its end (ZERO: also for a lane that starts
+// there): fetch8 is the memory access alone, so that several are in flight, and take8 what
+// follows it. No lane branches: a row's last, partial eight is read from the row's last eight
+// values and shifted down, since a lane that loaded its few values one by one would hold up the
+// wave for as many round trips.
+template <class T, Edge EDGE>
 __device__ __forceinline__ Raw<T> fetch8(const T* __restrict__ row, int64_t c, int64_t d) {
-  if (!NARROW) {
-    const int64_t at = c < d - 8 ? c : d - 8;
+  if (EDGE != kNarrow) {
+    const int64_t at = EDGE == kFull || c < d - 8 ? c : d - 8;
     return __builtin_bit_cast(Raw<T>, *reinterpret_cast<const Eight<T>*>(row + at));
   }
   Eight<T> e;
@@ -51,49 +56,56 @@ __device__ __forceinline__ Raw<T> fetch8(const T* __restrict__ row, int64_t c, i
   return __builtin_bit_cast(Raw<T>, e);
 }
 
-template <class T, bool NARROW>
+template <class T, Edge EDGE, bool ZERO = true>
 __device__ __forceinline__ void take8(Raw<T> t, int64_t c, int64_t d, float (&v)[8]) {
   constexpr int kWords = 2 * sizeof(T), kPer = 4 / sizeof(T);  // elements a word
-  if (!NARROW && (d & 7)) {
-    const int s = c > d - 8 ? (int)(c - d) & 7 : 0;
+  if (EDGE == kRagged) {
+    if (d & 7) {
+      const int s = c > d - 8 ? (int)(c - d) & 7 : 0;
 #pragma unroll
-    for (int bit = 4; bit >= 1; bit >>= 1) {
+      for (int bit = 4; bit >= 1; bit >>= 1) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        uint32_t from;
-        if (bit >= kPer) {
-          from = i + bit / kPer < kWords ? t.w[i + bit / kPer] : 0u;
-        } else {  // half a word
-          from = (t.w[i] >> 16) | (i + 1 < kWords ? t.w[i + 1] << 16 : 0u);
+        for (int i = 0; i < kWords; ++i) {
+          uint32_t from;
+          if (bit >= kPer) {
+            from = i + bit / kPer < kWords ? t.w[i + bit / kPer] : 0u;
+          } else {  // half a word
+            from = (t.w[i] >> 16) | (i + 1 < kWords ? t.w[i + 1] << 16 : 0u);
+          }
+          t.w[i] = s & bit ? from : t.w[i];
         }
-        t.w[i] = s & bit ? from : t.w[i];
       }
+    }
+    if (ZERO) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) t.w[i] = c < d ? t.w[i] : 0u;
     }
   }
   const Eight<T> e = __builtin_bit_cast(Eight<T>, t);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (NARROW ? c == 0 && i < d : c < d) ? (float)e.v[i] : 0.f;
+  for (int i = 0; i < 8; ++i)
+    v[i] = EDGE != kNarrow || (c == 0 && i < d) ? (float)e.v[i] : 0.f;
 }
 
 // Both at once, for any width.
 template <class T>
 __device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c, int64_t d,
                                       float (&v)[8]) {
-  if (d >= 8) take8<T, false>(fetch8<T, false>(row, c, d), c, d, v);
-  else take8<T, true>(fetch8<T, true>(row, c, d), c, d, v);
+  if (d >= 8) take8<T, kRagged>(fetch8<T, kRagged>(row, c, d), c, d, v);
+  else take8<T, kNarrow>(fetch8<T, kNarrow>(row, c, d), c, d, v);
 }
 
-template <class T>
+template <class T, Edge EDGE = kRagged>
 __device__ __forceinline__ void store8(T* __restrict__ row, int64_t c, int64_t d,
                                        const float (&v)[8]) {
   T* p = row + c;
-  const int64_t n = d - c;
-  if (n >= 8) {
+  if (EDGE == kFull || d - c >= 8) {
     Eight<T> t;
 #pragma unroll
     for (int e = 0; e < 8; ++e) t.v[e] = (T)v[e];
     *reinterpret_cast<Eight<T>*>(p) = t;
   } else {
+    const int n = (int)(d - c);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e < n) p[e] = (T)v[e];
@@ -136,6 +148,13 @@ __device__ __forceinline__ void philox(uint64_t key, uint32_t c0, uint64_t row, 
     k1 += 0xBB67AE85u;
   }
   w[0] = x0, w[1] = x1, w[2] = x2, w[3] = x3;
+}
+
+// v * f, and 0 where f is 0 whatever v is (an infinity, a NaN).
+__device__ __forceinline__ float masked(float v, float f) {
+  float r;  // the multiplication in which 0 times anything is 0: one instruction for three
+  asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(v), "v"(f));
+  return r;
 }
 
 // f[e] = scale where value e of block (row, cb) is kept, 0 where it is dropped.
