@@ -167,6 +167,16 @@ __device__ __forceinline__ void form_h(const NormIn& in, uint64_t key, const In&
   }
 }
 
+// 1 / sqrt(v): the hardware's estimate (1 ulp) and one Newton step, over the range where neither
+// leaves the normal numbers; the exact root and quotient, some thirty instructions, elsewhere.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  if (v > 1e-30f && v < 1e30f) {
+    const float r = __builtin_amdgcn_rsqf(v);
+    return fmaf(r, 0.5f * fmaf(-v * r, r, 1.f), r);
+  }
+  return 1.f / __builtin_sqrtf(v);
+}
+
 // h -> u in place; returns r. Behind the row's end u is finite where the row is (the gradients
 // there are 0, and nothing of it is stored).
 template <int TPR, int NV, Edge EDGE>
@@ -196,7 +206,7 @@ __device__ __forceinline__ float normalize(const NormIn& in, int t, float (&h)[N
   row_sum2<TPR>(s1, s2, red);
   const float off = s1 * inv;
   const float var = fmaxf(fmaf(-off, off, s2 * inv), 0.f);
-  const float r = 1.f / __builtin_sqrtf(var + in.eps);
+  const float r = inv_sqrt(var + in.eps);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -208,33 +218,41 @@ template <class T, int TPR, int NV, Edge EDGE, bool PLAIN>
 __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock) void norm_forward_kernel(
     NormIn in, T* __restrict__ y, int64_t ldy, T* __restrict__ hout, int64_t ldh) {
   constexpr int kBlock = TPR > kNormBlock ? TPR : kNormBlock;
+  constexpr bool HELD = NV == 1;  // w and b stay in registers over a lane group's rows
   __shared__ float red[2 * kBlock / 64];
   const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * (kBlock / TPR) + threadIdx.x / TPR;
-  if (row >= in.rows) return;  // whole rows only: the lanes of a row leave together
-  RowIn<T, TPR, NV, EDGE, PLAIN ? 1 : 2> raw;
-  raw.fetch(0, in.x, in.ldx, row, in.d, t);
-  if (!PLAIN) raw.fetch(PLAIN ? 0 : 1, in.res, in.ldr, row, in.d, t);
-  float h[NV][8], none[NV][8];
-  form_h<PLAIN, false, TPR, NV>(in, in.dropping ? drop_key(in.drop) : 0, raw, row, t, h,
-                                none);
-  if (hout) {
+  const uint64_t key = in.dropping ? drop_key(in.drop) : 0;
+  float w[8], b[8];
+  auto params = [&](int j) {
+    const int64_t c = (int64_t)(j * TPR + t) * 8;
+    load_param<T, EDGE>(in.w, in.w_f32, c, in.d, 1.f, w);
+    load_param<T, EDGE>(in.b, in.w_f32, c, in.d, 0.f, b);
+  };
+  const int64_t stride = (int64_t)gridDim.x * (kBlock / TPR);
+  int64_t row = (int64_t)blockIdx.x * (kBlock / TPR) + threadIdx.x / TPR;
+  if (HELD && row < in.rows) params(0);
+  for (; row < in.rows; row += stride) {  // the lanes of a row leave together
+    RowIn<T, TPR, NV, EDGE, PLAIN ? 1 : 2> raw;
+    raw.fetch(0, in.x, in.ldx, row, in.d, t);
+    if (!PLAIN) raw.fetch(PLAIN ? 0 : 1, in.res, in.ldr, row, in.d, t);
+    float h[NV][8], none[NV][8];
+    form_h<PLAIN, false, TPR, NV>(in, key, raw, row, t, h, none);
+    if (hout) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int64_t c = (int64_t)(j * TPR + t) * 8;
+        store8<T, EDGE>(hout + row * ldh, c, in.d, h[j]);
+      }
+    }
+    normalize<TPR, NV, EDGE>(in, t, h, red);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t c = (int64_t)(j * TPR + t) * 8;
-      store8<T, EDGE>(hout + row * ldh, c, in.d, h[j]);
+      if (!HELD) params(j);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[j][e] = fmaf(h[j][e], w[e], b[e]);
+      store8<T, EDGE>(y + row * ldy, c, in.d, h[j]);
     }
-  }
-  normalize<TPR, NV, EDGE>(in, t, h, red);
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int64_t c = (int64_t)(j * TPR + t) * 8;
-    float w[8], b[8];
-    load_param<T, EDGE>(in.w, in.w_f32, c, in.d, 1.f, w);
-    load_param<T, EDGE>(in.b, in.w_f32, c, in.d, 0.f, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[j][e] = fmaf(h[j][e], w[e], b[e]);
-    store8<T, EDGE>(y + row * ldy, c, in.d, h[j]);
   }
 }
 
@@ -281,6 +299,8 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
   };
   In next;
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
+  float w[8];
+  if (NV == 1) load_param<T, EDGE>(in.w, in.w_f32, t * 8, in.d, 1.f, w);
   if (AHEAD && row < in.rows) fetch(next, row);
   for (; row < in.rows; row += stride) {
     In raw;
@@ -297,9 +317,8 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
     if (kWhenNeeded) raw.fetch(kDy, dy, lddy, row, in.d, t);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float w[8];
       raw.template take<true>(kDy, j, in.d, t, g[j]);
-      load_param<T, EDGE>(in.w, in.w_f32, (int64_t)(j * TPR + t) * 8, in.d, 1.f, w);
+      if (NV > 1) load_param<T, EDGE>(in.w, in.w_f32, (int64_t)(j * TPR + t) * 8, in.d, 1.f, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (LATE) {
@@ -363,7 +382,8 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
     for (int k = 0; k < 2; ++k) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) join[threadIdx.x * 8 + e] = k ? ab[LATE ? 0 : j][e] : aw[LATE ? 0 : j][e];
+      for (int e = 0; e < 8; ++e)
+        join[threadIdx.x * 8 + e] = k ? ab[LATE ? 0 : j][e] : aw[LATE ? 0 : j][e];
       __syncthreads();
       for (int i = threadIdx.x; i < TPR * 8; i += kBlock) {
         const int64_t c = (int64_t)j * TPR * 8 + i;
@@ -436,8 +456,9 @@ static int with_shape(int64_t d, bool plain, F&& f) {
 }
 
 // Rows a workgroup holds at a time, and workgroups of the backward pass: as many as are resident
-// together (four a CU, two where rows are wide), each with one partial row. 8192 x 4096 bf16, both
-// passes: 512 workgroups 105 us, 1024 111, 256 126; 2M x 64 fp32 block: 1024 966, 1280 1361.
+// together (by the registers four, three or two a CU), each with one partial row. 8192 x 4096
+// bf16, both passes: 768 workgroups 85.9 us, 512 88.5, 1024 96.3; 10 003 x 8192 fp32: 512 343, 768
+// 364; 2M x 64 fp32 block: 1024 966, 1280 1361.
 static int64_t rows_per_block(int64_t d) {
   int64_t r = 1;
   with_shape(d, false, [&](auto s) {
@@ -447,7 +468,7 @@ static int64_t rows_per_block(int64_t d) {
   return r;
 }
 static int64_t backward_blocks(int64_t rows, int64_t d) {
-  const int64_t b = ceil_div(rows, rows_per_block(d)), most = d <= 1024 ? 1024 : 512;
+  const int64_t b = ceil_div(rows, rows_per_block(d)), most = d <= 1024 ? 1024 : d <= 4096 ? 768 : 512;
   return b < most ? b : most;
 }
 
@@ -496,9 +517,14 @@ extern "C" int gnnrec_layer_norm_forward(int32_t dtype, int32_t wdtype, int64_t 
     return with_shape(d, is_plain(in), [&](auto s) {
       using S = decltype(s);
       constexpr int kBlock = S::tpr > kNormBlock ? S::tpr : kNormBlock;
+      // half-precision blocks are bound by instructions, and resident workgroups load w and b
+      // once (100 003 x 201 fp16 block, both passes: 118 -> 110 us); the others by memory, and
+      // one row a lane group keeps more of it in flight (2M x 64 fp32: 960 us, resident 1000)
+      const int64_t want = ceil_div(rows, kBlock / S::tpr);
+      const int64_t most = sizeof(T) == 2 && !S::plain ? 2048 : 0x7fffffff;
       hipLaunchKernelGGL((norm_forward_kernel<T, S::tpr, S::nv, S::edge, S::plain>),
-                         dim3((unsigned)ceil_div(rows, kBlock / S::tpr)), dim3(kBlock), 0,
-                         as_hip(stream), in, (T*)y, ldy, (T*)h, ldh);
+                         dim3((unsigned)(want < most ? want : most)),
+                         dim3(kBlock), 0, as_hip(stream), in, (T*)y, ldy, (T*)h, ldh);
       return check_launch("layer_norm_forward");
     });
   });
@@ -531,8 +557,9 @@ extern "C" int gnnrec_layer_norm_backward(int32_t dtype, int32_t wdtype, int64_t
         using S = decltype(s);
         constexpr int kBlock = S::tpr > kNormBlock ? S::tpr : kNormBlock;
         hipLaunchKernelGGL((norm_backward_kernel<T, S::tpr, S::nv, S::edge, S::plain>),
-                           dim3((unsigned)blocks), dim3(kBlock), 0, as_hip(stream), in, (const T*)dy, lddy, (const T*)dh,
-                           lddh, (T*)dx, lddx, (T*)dres, lddr, dw || db ? work : nullptr);
+                           dim3((unsigned)blocks), dim3(kBlock), 0, as_hip(stream), in,
+                           (const T*)dy, lddy, (const T*)dh, lddh, (T*)dx, lddx,
+                           (T*)dres, lddr, dw || db ? work : nullptr);
         return check_launch("layer_norm_backward");
       });
     });
