@@ -183,26 +183,23 @@ template <int TPR, int NV, Edge EDGE>
 __device__ __forceinline__ float normalize(const NormIn& in, int t, float (&h)[NV][8],
                                            float* red) {
   const float inv = 1.f / (float)in.d;
+  const int n = (int)in.d - t * 8;  // block j of this lane has n - j TPR 8 values in the row
   float s = 0.f, unused = 0.f;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int n = (int)in.d - (j * TPR + t) * 8;
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += EDGE == kFull || e < n ? h[j][e] : 0.f;
-  }
+    for (int e = 0; e < 8; ++e) s += EDGE == kFull || e < n - j * TPR * 8 ? h[j][e] : 0.f;
   row_sum2<TPR>(s, unused, red);
   const float mean = s * inv;
   float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int n = (int)in.d - (j * TPR + t) * 8;
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      h[j][e] = EDGE == kFull || e < n ? h[j][e] - mean : 0.f;
+      h[j][e] = EDGE == kFull || e < n - j * TPR * 8 ? h[j][e] - mean : 0.f;
       s1 += h[j][e];
       s2 = fmaf(h[j][e], h[j][e], s2);
     }
-  }
   row_sum2<TPR>(s1, s2, red);
   const float off = s1 * inv;
   const float var = fmaxf(fmaf(-off, off, s2 * inv), 0.f);
@@ -422,9 +419,9 @@ __global__ __launch_bounds__(kSumCols* kSumSlices) void norm_sum_kernel(
 }
 
 // Lanes a row and blocks a lane by the row's width (blocks of eight columns): one wave holds up
-// to 1024 columns, wider rows take a workgroup. Narrow shapes have an instance for rows that fill
-// every lane (64, 128, 256, 512, 1024 columns: no masks), wide ones for the norm alone (no
-// registers for a residual and a mask).
+// to 1024 columns, wider rows take a workgroup. Rows that fill every lane (a power of two from 64
+// columns on) have an instance without masks, and rows of a workgroup one for the norm alone,
+// without registers for a residual and a mask.
 template <int TPR, int NV, Edge EDGE, bool PLAIN>
 struct Shape {
   static constexpr int tpr = TPR, nv = NV;
@@ -437,8 +434,9 @@ static int one_wave(int64_t d, F&& f) {
                            : f(Shape<TPR, NV, kRagged, false>{});
 }
 template <int TPR, int NV, class F>
-static int workgroup(bool plain, F&& f) {
-  return plain ? f(Shape<TPR, NV, kRagged, true>{}) : f(Shape<TPR, NV, kRagged, false>{});
+static int workgroup(int64_t d, bool plain, F&& f) {
+  if (!plain) return f(Shape<TPR, NV, kRagged, false>{});
+  return d == TPR * NV * 8 ? f(Shape<TPR, NV, kFull, true>{}) : f(Shape<TPR, NV, kRagged, true>{});
 }
 template <class F>
 static int with_shape(int64_t d, bool plain, F&& f) {
@@ -449,10 +447,10 @@ static int with_shape(int64_t d, bool plain, F&& f) {
   if (nb <= 32) return one_wave<32, 1>(d, f);
   if (nb <= 64) return one_wave<64, 1>(d, f);
   if (nb <= 128) return one_wave<64, 2>(d, f);
-  if (nb <= 256) return workgroup<256, 1>(plain, f);
-  if (nb <= 512) return workgroup<256, 2>(plain, f);
-  if (nb <= 1024) return workgroup<512, 2>(plain, f);
-  return workgroup<1024, 2>(plain, f);
+  if (nb <= 256) return workgroup<256, 1>(d, plain, f);
+  if (nb <= 512) return workgroup<256, 2>(d, plain, f);
+  if (nb <= 1024) return workgroup<512, 2>(d, plain, f);
+  return workgroup<1024, 2>(d, plain, f);
 }
 
 // Rows a workgroup holds at a time, and workgroups of the backward pass: as many as are resident
@@ -468,7 +466,8 @@ static int64_t rows_per_block(int64_t d) {
   return r;
 }
 static int64_t backward_blocks(int64_t rows, int64_t d) {
-  const int64_t b = ceil_div(rows, rows_per_block(d)), most = d <= 1024 ? 1024 : d <= 4096 ? 768 : 512;
+  const int64_t b = ceil_div(rows, rows_per_block(d));
+  const int64_t most = d <= 1024 ? 1024 : d <= 4096 ? 768 : 512;
   return b < most ? b : most;
 }
 
