@@ -23,6 +23,7 @@ A dropped value is 0 whatever x holds there, also an infinity or a NaN.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
@@ -73,6 +74,18 @@ def rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
                      "tensor")
 
 
+def _empty_rows(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape and type."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+@lru_cache(maxsize=256)
+def _norm_work_floats(rows: int, d: int) -> int:
+    return _lib.lib().gnnrec_layer_norm_work_floats(rows, d)
+
+
 def _dense_rows(t: Optional[torch.Tensor]):
     """(tensor, row stride) in a backward pass, of an incoming gradient (which may have any
     layout: an expanded scalar) or of a saved tensor (which a saved-tensor hook may have laid
@@ -85,9 +98,7 @@ def _dense_rows(t: Optional[torch.Tensor]):
     return t, t.shape[-1]
 
 
-def _same(what: str, x: torch.Tensor, t: Optional[torch.Tensor], name: str) -> None:
-    if t is None:
-        return
+def _same(what: str, x: torch.Tensor, t: torch.Tensor, name: str) -> None:
     if t.device != x.device:
         raise ValueError(f"{what}: {name} on {t.device}, x on {x.device}")
     if t.dtype != x.dtype:
@@ -129,7 +140,7 @@ def _once(backward):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ldx, rows, p, seed_t, site, row0, slope, seed):
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y = _empty_rows(x)
         d = x.shape[-1]
         launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, x.data_ptr(),
                ldx, y.data_ptr(), d, p, seed, ptr(seed_t), site, row0, slope)
@@ -143,7 +154,7 @@ class _Dropout(torch.autograd.Function):
         rows, p, site, row0, slope, seed = ctx.cfg
         x, ldx = _dense_rows(x)
         dy, lddy = _dense_rows(dy)
-        dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+        dx = _empty_rows(dy)
         d = dy.shape[-1]
         launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x), ldx,
                dy.data_ptr(), lddy, dx.data_ptr(), d, p, seed, ptr(seed_t), site, row0, slope)
@@ -167,7 +178,7 @@ class _NormBlock(torch.autograd.Function):
     def forward(ctx, keep_h, x, ldx, rows, res, ldr, w, b, eps, p, seed_t, site, row0, slope,
                 seed):
         ctx.set_materialize_grads(False)
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y = _empty_rows(x)
         h = torch.empty_like(y) if keep_h else None
         d = x.shape[-1]
         t = _lib.DTYPES[x.dtype]
@@ -195,14 +206,13 @@ class _NormBlock(torch.autograd.Function):
         dy, lddy = _dense_rows(dy)
         dh, lddh = _dense_rows(dh)
         d = x.shape[-1]
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[1] else None
-        dres = torch.empty_like(x, memory_format=torch.contiguous_format) if need[4] else None
+        dx = _empty_rows(x) if need[1] else None
+        dres = _empty_rows(x) if need[4] else None
         dw = torch.empty_like(w) if need_w else None
         db = x.new_empty(d, dtype=b_dtype) if need_b else None
         work = None
         if need_w or need_b:
-            work = x.new_empty(_lib.lib().gnnrec_layer_norm_work_floats(rows, d),
-                               dtype=torch.float32)
+            work = x.new_empty(_norm_work_floats(rows, d), dtype=torch.float32)
         launch("gnnrec_layer_norm_backward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res),
                ldr, ptr(w), eps, p, seed, ptr(seed_t), site, row0, slope, dy.data_ptr(), lddy,
                ptr(dh), lddh, ptr(dx), d, ptr(dres), d, ptr(dw), ptr(db), ptr(work))
