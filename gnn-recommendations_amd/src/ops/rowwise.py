@@ -20,6 +20,9 @@ draws what one device would, and a second dropout of the same step takes another
 is an int or a one-element int64 tensor on the table's device; a captured graph reads the tensor
 on every replay, so `seed.add_(1)` between replays (or captured in front) gives new masks.
 A dropped value is 0 whatever x holds there, also an infinity or a NaN.
+
+Forward and backward may be captured into a graph. As for any torch operator, no eager autograd
+graph of the same leaves may be alive while a backward pass is captured.
 """
 from __future__ import annotations
 
@@ -39,7 +42,9 @@ Seed = Union[int, torch.Tensor]
 
 _ENTRIES: dict = {}
 _current_device = torch.cuda.current_device
-_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream, less the objects
+# torch.cuda.current_stream(i).cuda_stream without the objects around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def launch(name: str, device: torch.device, *args) -> None:

@@ -49,6 +49,27 @@ def test_users(cuda, dtype, m):
         _check(x, _table(n, k, seed=1), what=f"{m}x{n}x{k}")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m", [1, 4, 5, 20])
+@pytest.mark.parametrize("n,k", [(16383, 257), (16384, 257), (65535, 64), (65536, 64),
+                                 (65537, 33), (65600, 96), (65537, 150), (65600, 192),
+                                 (65601, 224), (17000, 2048), (16400, 2080), (70000, 300),
+                                 (4100, 4096), (200, 8192), (50, 16000)])
+def test_ways_of_sharing_out(cuda, dtype, m, n, k):
+    """Both sides of every border between the kernels, and every number of trailing groups with
+    one tile and with four; the table's rows repeat, so the oracle stays small."""
+    t = _table(256, k, seed=2)
+    rep = -(-n // 256)
+    big = ops.Q4Table(t.codes.repeat(rep, 1)[:n], t.scale.repeat(rep, 1)[:n], k)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).to(dtype).cuda()
+    got = ops.q4_matmul(x, big)
+    _check(x, t, out=got[:, :256].contiguous() if n >= 256 else ops.q4_matmul(x, t))
+    first = got[:, :256] if n >= 256 else got
+    for r in range(0, n, 256):
+        part = got[:, r:r + 256]
+        assert torch.equal(part, first[:, :part.shape[1]]), r
+
+
 def test_users_beyond_a_grid_row(cuda):
     x = torch.randn(3000, 64, generator=torch.Generator().manual_seed(0)).cuda()
     _check(x, _table(90, 64))

@@ -203,8 +203,9 @@ def test_far_mean_and_constant_rows(cuda):
         assert torch.equal(y, b.expand(5, 300))
 
 
-def test_non_finite_rows_stay_in_their_row(cuda):
-    x = _randn(64, 48)
+@pytest.mark.parametrize("d", [48, 64, 201, 1500, 4096])
+def test_non_finite_rows_stay_in_their_row(cuda, d):
+    x = _randn(64, d)
     want = ops.layer_norm(x)
     for bad in (float("inf"), float("nan")):
         z = x.clone()
@@ -274,6 +275,16 @@ def test_views_and_ranks(cuda):
         _check_block(60, 64, F32, F32, 0.1, 0.2, True, True, x=x.detach())
     x = _randn(3, 4, 5, 64)
     assert torch.equal(ops.layer_norm(x), ops.layer_norm(x.view(60, 64)).view_as(x))
+    for shape in ((64,), (3, 4, 5, 64)):          # gradients of other ranks
+        x, dy = _randn(*shape).requires_grad_(), _randn(*shape, seed=1)
+        y, h = ops.dropout_add_layer_norm(x, x.detach(), None, None, 0.2, 3, negative_slope=0.2)
+        got = torch.autograd.grad((y, h, ops.dropout(x, 0.2, 3)), x, (dy, dy, dy))[0]
+        x2 = x.detach().view(-1, 64).requires_grad_()
+        y, h = ops.dropout_add_layer_norm(x2, x2.detach(), None, None, 0.2, 3,
+                                          negative_slope=0.2)
+        d2 = dy.view(-1, 64)
+        want = torch.autograd.grad((y, h, ops.dropout(x2, 0.2, 3)), x2, (d2, d2, d2))[0]
+        assert got.shape == shape and torch.equal(got.view(-1, 64), want)
     res = _randn(1, 64).requires_grad_()          # one residual row for all
     x = _randn(60, 64, seed=8)
     y, h = ops.dropout_add_layer_norm(x, res.expand(60, 64), None, None, 0.0, 0)
@@ -309,6 +320,24 @@ def test_no_rows(cuda):
     y = ops.layer_norm(x, w, b)
     dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
     assert y.shape == dx.shape == (0, 64) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("scale,eps", [(1e-12, 1e-5), (1e-12, 0.0), (1e-18, 0.0), (1e8, 1e-5),
+                                       (3e15, 1e-5), (1e18, 0.0)])
+def test_variances_over_the_range(cuda, scale, eps):
+    """1 / sqrt at both ends of what fp32 holds, within the estimate's range and outside it (the
+    exact root there). Products below 2^-126 keep 2^-149, which at 1e-18 (variance 1e-36) is
+    1e-9 of them."""
+    x = _randn(20, 128) * scale
+    y = ops.layer_norm(x, eps=eps)
+    f = torch.ones(20, 128, dtype=torch.float64)
+    want, bound = R.block(x.cpu(), None, None, None, eps, f, 1.0)["y"]
+    R.assert_close(y, want, bound, f"{scale} {eps}")
+    # beyond it: a variance of zero without eps has no norm; an overflowing one gives 0
+    z = ops.layer_norm(torch.full((1, 8), 3.0, device="cuda"), eps=0.0)
+    assert z.isnan().all()
+    big = torch.tensor([[3e38, -3e38] * 32], device="cuda")
+    assert not ops.layer_norm(big).any()
 
 
 def test_equal_inputs_give_equal_bits(cuda):
