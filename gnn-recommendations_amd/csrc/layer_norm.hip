@@ -17,6 +17,10 @@
 // dw and db: every workgroup sums its rows in registers, joins its lane groups through LDS and
 // writes one partial row; a second launch adds the partial rows, each column in a fixed order
 // (no atomics: equal inputs give equal bits).
+//
+// fp32 tables are bound by memory (the block on 2M x 64: forward 187 us, 5.5 TB/s, backward 302 us,
+// 5.1, sums 6 us); half-precision blocks by instructions, most of them the generator's and the
+// conversions' (100 003 x 201 fp16: 38, 61 and 7 us, 62 % of the VALU's cycles busy forward).
 #include <type_traits>
 
 #include "rowwise.h"

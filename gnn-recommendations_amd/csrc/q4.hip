@@ -6,6 +6,10 @@
 //   value[r, c] = e2m1(code[r, c]) * scale[r, c / 32]
 //   out[i, r]   = sum over groups g of scale[r, g] * (sum over c in g of x[i, c] e2m1(code[r, c]))
 // E2M1 is the 4-bit type that this hardware converts by itself (two codes an instruction).
+//
+// All of it is bound by the table's bytes: one user against 1M x 64 9.6 us (4.2 TB/s), 16 users
+// against 1M x 256 bf16 48 us (3.7), 8192 x 8192 and one user 16 us (2.3: latency of two rounds of
+// loads); the quantiser 1M x 64 fp32 66 us (4.4).
 #include <type_traits>
 
 #include "rowwise.h"

@@ -1,11 +1,16 @@
 """The row-wise operators inside the framework's own paths: NGCF's counter-based dropout and
 layer norm, ranking against 4-bit items, and a run of them together."""
+import os
+
 import numpy as np
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 import torch.nn.functional as F
 
 import rowwise_ref as R
+from test_distributed import _free_port, cpu_ngcf_layer
 from test_models import torch_adj
 
 from src import ops
@@ -78,6 +83,42 @@ def test_cpu_forward_with_layer_norm(cls):
     assert all(p.grad is not None for p in m.layers.parameters())
 
 
+def _shard_worker(rank, world, port, q):
+    from src.ops.distributed import DistributedGraph, ngcf_forward_dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        g, adj = _graph()
+        with torch.no_grad():
+            got = []
+            for cls in (NGCF, NGCFGroupShuffle):
+                m = _model(cls, layer_norm=True).eval()
+                dg = DistributedGraph(g, rank, world, "cpu")
+                whole = ngcf_forward_dist(dg, m, dg.pad_table(m._initial_table()),
+                                          layer_fn=cpu_ngcf_layer, gather_output=True)
+                got.append((whole.numpy(), torch.cat(m(adj)).numpy()))
+            if rank == 0:
+                q.put(got)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_sharded_forward_with_layer_norm():
+    """Two ranks: the norm is row-local, so the shards give the rows of one device."""
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = _free_port()
+    procs = [ctx.Process(target=_shard_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = q.get(timeout=120)
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    for whole, single in got:     # the stand-in layer sums in another order: fp32, three layers
+        np.testing.assert_allclose(whole, single, rtol=1e-4, atol=1e-4)
+
+
 def test_evaluator_refuses():
     with pytest.raises(ValueError, match="ROCm device"):
         Evaluator(device=torch.device("cpu"), item_bits=4)
@@ -148,6 +189,11 @@ def test_ngcf_layer_norm_inference(cuda, cls):
         fast = torch.cat(m(g))
     slow = torch.cat(m(g)).detach()
     torch.testing.assert_close(fast, slow, rtol=1e-4, atol=1e-5)
+    from src.ops.distributed import DistributedGraph, ngcf_forward_dist
+    with torch.no_grad():
+        dg = DistributedGraph(g, 0, 1, cuda)
+        local = ngcf_forward_dist(dg, m, dg.pad_table(m._initial_table()))
+    assert torch.equal(local[:800], fast)
     cpu = _model(cls, layer_norm=True)
     cpu.load_state_dict({k: v.cpu() for k, v in m.state_dict().items()})
     with torch.no_grad():
