@@ -114,7 +114,8 @@ def _same(what: str, x: torch.Tensor, t: torch.Tensor, name: str) -> None:
 
 def _drop_args(what: str, x: torch.Tensor, p: float, seed: Seed, site: int, row0: int,
                negative_slope: float):
-    """(p, seed tensor or None, site, row0, slope, host seed), checked."""
+    """(seed tensor or None, (p, host seed), (site, row0, slope)), checked: the mask's arguments
+    of the C entries, around the seed's address."""
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"{what}: p must be between 0 and 1, got {p}")
@@ -130,7 +131,16 @@ def _drop_args(what: str, x: torch.Tensor, p: float, seed: Seed, site: int, row0
         if seed.device != x.device:
             raise ValueError(f"{what}: seed on {seed.device}, x on {x.device}")
         tensor, seed = seed, 0
-    return p, tensor, int(site), int(row0), float(negative_slope), int(seed) & (2 ** 64 - 1)
+    return (tensor, (p, int(seed) & (2 ** 64 - 1)),
+            (int(site), int(row0), float(negative_slope)))
+
+
+_NO_MASK = (None, (0.0, 0), (0, 0, 1.0))
+
+
+def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether autograd records a call with these inputs (otherwise its bookkeeping is skipped)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _once(backward):
@@ -142,28 +152,35 @@ def _once(backward):
     return staticmethod(wrapped)
 
 
+def _dropout_forward(x, ldx, rows, mask):
+    seed_t, pre, post = mask
+    y = _empty_rows(x)
+    d = x.shape[-1]
+    launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, x.data_ptr(), ldx,
+           y.data_ptr(), d, *pre, ptr(seed_t), *post)
+    return y
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, ldx, rows, p, seed_t, site, row0, slope, seed):
-        y = _empty_rows(x)
-        d = x.shape[-1]
-        launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, x.data_ptr(),
-               ldx, y.data_ptr(), d, p, seed, ptr(seed_t), site, row0, slope)
-        ctx.save_for_backward(x if slope != 1.0 else None, seed_t)
-        ctx.cfg = (rows, p, site, row0, slope, seed)
+    def forward(ctx, x, ldx, rows, mask):
+        y = _dropout_forward(x, ldx, rows, mask)
+        seed_t, pre, post = mask
+        ctx.save_for_backward(x if post[2] != 1.0 else None, seed_t)
+        ctx.cfg = (rows, pre, post)
         return y
 
     @_once
     def backward(ctx, dy):
         x, seed_t = ctx.saved_tensors
-        rows, p, site, row0, slope, seed = ctx.cfg
+        rows, pre, post = ctx.cfg
         x, ldx = _dense_rows(x)
         dy, lddy = _dense_rows(dy)
         dx = _empty_rows(dy)
         d = dy.shape[-1]
         launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x), ldx,
-               dy.data_ptr(), lddy, dx.data_ptr(), d, p, seed, ptr(seed_t), site, row0, slope)
-        return dx, None, None, None, None, None, None, None, None
+               dy.data_ptr(), lddy, dx.data_ptr(), d, *pre, ptr(seed_t), *post)
+        return dx, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: Seed, *, site: int = 0, row0: int = 0,
@@ -172,38 +189,39 @@ def dropout(x: torch.Tensor, p: float, seed: Seed, *, site: int = 0, row0: int =
     the module's text for the mask, `seed`, `site` and `row0`. p = 1 drops everything, p = 0
     nothing. p counts in steps of 1 / 65536, and the scale goes by the step used."""
     x2 = rows_of(x, "dropout")
-    return _Dropout.apply(x, x2.stride(0), x2.shape[0], *_drop_args("dropout", x, p, seed, site, row0, negative_slope))
+    mask = _drop_args("dropout", x, p, seed, site, row0, negative_slope)
+    call = _Dropout.apply if _tracked(x) else _dropout_forward
+    return call(x, x2.stride(0), x2.shape[0], mask)
+
+
+def _norm_forward(x, res, w, b, cfg):
+    """(y, h) = (LN(h) w + b, h), h = residual + dropout(leaky(x)); h is None without `keep_h`
+    (layer_norm alone: h is x)."""
+    keep_h, rows, ldx, ldr, t, wt, eps, (seed_t, pre, post) = cfg
+    y = _empty_rows(x)
+    h = torch.empty_like(y) if keep_h else None
+    d = x.shape[-1]
+    launch("gnnrec_layer_norm_forward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res), ldr,
+           ptr(w), ptr(b), eps, *pre, ptr(seed_t), *post, y.data_ptr(), d, ptr(h), d)
+    return y, h
 
 
 class _NormBlock(torch.autograd.Function):
-    """(y, h) = (LN(h) w + b, h), h = residual + dropout(leaky(x)); h is None without `keep_h`
-    (layer_norm alone: h is x)."""
-
     @staticmethod
-    def forward(ctx, keep_h, x, ldx, rows, res, ldr, w, b, eps, p, seed_t, site, row0, slope,
-                seed):
+    def forward(ctx, x, res, w, b, cfg):
         ctx.set_materialize_grads(False)
-        y = _empty_rows(x)
-        h = torch.empty_like(y) if keep_h else None
-        d = x.shape[-1]
-        t = _lib.DTYPES[x.dtype]
-        wt = t if w is None and b is None else _lib.DTYPES[(b if w is None else w).dtype]
-        launch("gnnrec_layer_norm_forward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res),
-               ldr, ptr(w), ptr(b), eps, p, seed, ptr(seed_t), site, row0, slope, y.data_ptr(), d,
-               ptr(h), d)
-        ctx.save_for_backward(x, res, w, seed_t)
-        ctx.cfg = (rows, t, wt, eps, p, site, row0, slope, seed,
-                   b.dtype if b is not None else None)
-        return y, h
+        ctx.save_for_backward(x, res, w, cfg[7][0])
+        ctx.cfg = cfg
+        ctx.b_dtype = b.dtype if b is not None else None
+        return _norm_forward(x, res, w, b, cfg)
 
     @_once
     def backward(ctx, dy, dh):
         x, res, w, seed_t = ctx.saved_tensors
-        rows, t, wt, eps, p, site, row0, slope, seed, b_dtype = ctx.cfg
-        need = ctx.needs_input_grad
-        need_w, need_b = need[6], need[7]
+        _, rows, _, _, t, wt, eps, (_, pre, post) = ctx.cfg
+        need_x, need_r, need_w, need_b, _ = ctx.needs_input_grad
         if dy is None and dh is None:
-            return (None,) * 15
+            return None, None, None, None, None
         if dy is None:      # only h was used: nothing passes through the norm
             dy = torch.zeros_like(dh)
         x, ldx = _dense_rows(x)
@@ -211,17 +229,30 @@ class _NormBlock(torch.autograd.Function):
         dy, lddy = _dense_rows(dy)
         dh, lddh = _dense_rows(dh)
         d = x.shape[-1]
-        dx = _empty_rows(x) if need[1] else None
-        dres = _empty_rows(x) if need[4] else None
+        dx = _empty_rows(x) if need_x else None
+        dres = _empty_rows(x) if need_r else None
         dw = torch.empty_like(w) if need_w else None
-        db = x.new_empty(d, dtype=b_dtype) if need_b else None
+        db = x.new_empty(d, dtype=ctx.b_dtype) if need_b else None
         work = None
         if need_w or need_b:
             work = x.new_empty(_norm_work_floats(rows, d), dtype=torch.float32)
         launch("gnnrec_layer_norm_backward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res),
-               ldr, ptr(w), eps, p, seed, ptr(seed_t), site, row0, slope, dy.data_ptr(), lddy,
-               ptr(dh), lddh, ptr(dx), d, ptr(dres), d, ptr(dw), ptr(db), ptr(work))
-        return (None, dx, None, None, dres, None, dw, db) + (None,) * 7
+               ldr, ptr(w), eps, *pre, ptr(seed_t), *post, dy.data_ptr(), lddy, ptr(dh), lddh,
+               ptr(dx), d, ptr(dres), d, ptr(dw), ptr(db), ptr(work))
+        return dx, dres, dw, db, None
+
+
+def _norm_block(what, keep_h, x, res, w, b, eps, mask):
+    ldx, rows = _norm_args(what, x, w, b, eps)
+    ldr = 0
+    if res is not None:
+        _same(what, x, res, "residual")
+        ldr = rows_of(res, what).stride(0)
+    t = _lib.DTYPES[x.dtype]
+    wt = t if w is None and b is None else _lib.DTYPES[(b if w is None else w).dtype]
+    cfg = (keep_h, rows, ldx, ldr, t, wt, float(eps), mask)
+    call = _NormBlock.apply if _tracked(x, res, w, b) else _norm_forward
+    return call(x, res, w, b, cfg)
 
 
 def _norm_args(what: str, x: torch.Tensor, weight, bias, eps: float):
@@ -252,9 +283,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     MAX_NORM_WIDTH values; var divides by their number). weight and bias: x's dtype or float32,
     either may be None. Gradients of x, weight and bias; the weight's and the bias's are summed
     over all rows in fp32 in a fixed order."""
-    ldx, rows = _norm_args("layer_norm", x, weight, bias, eps)
-    return _NormBlock.apply(False, x, ldx, rows, None, 0, weight, bias, float(eps), 0.0, None, 0,
-                            0, 1.0, 0)[0]
+    return _norm_block("layer_norm", False, x, None, weight, bias, eps, _NO_MASK)[0]
 
 
 def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
@@ -266,10 +295,5 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor],
     + bias; returns (y, h). residual None: h = dropout(LeakyReLU(x)). The mask is dropout()'s for
     the same p, seed, site and row0; the norm is layer_norm()'s, of the unrounded h."""
     what = "dropout_add_layer_norm"
-    ldx, rows = _norm_args(what, x, weight, bias, eps)
-    ldr = 0
-    if residual is not None:
-        _same(what, x, residual, "residual")
-        ldr = rows_of(residual, what).stride(0)
-    return _NormBlock.apply(True, x, ldx, rows, residual, ldr, weight, bias, float(eps),
-                            *_drop_args(what, x, p, seed, site, row0, negative_slope))
+    mask = _drop_args(what, x, p, seed, site, row0, negative_slope)
+    return _norm_block(what, True, x, residual, weight, bias, eps, mask)

@@ -20,9 +20,9 @@ from src.models import NGCF, NGCFGroupShuffle
 from src.ops import CsrGraph
 
 
-def _model(cls=NGCF, seed=5, **kw):
+def _model(cls=NGCF, seed=5, sizes=(64, 64, 32), **kw):
     torch.manual_seed(seed)
-    m = cls(300, 500, embedding_dim=64, layer_sizes=[64, 64, 32], dropout=0.1, init_scale=0.3,
+    m = cls(300, 500, embedding_dim=64, layer_sizes=list(sizes), dropout=0.1, init_scale=0.3,
             **kw)
     with torch.no_grad():
         for layer in m.layers:
@@ -181,7 +181,7 @@ def test_ngcf_seed_comes_from_torch(cuda):
 @pytest.mark.parametrize("cls", [NGCF, NGCFGroupShuffle])
 def test_ngcf_layer_norm_inference(cuda, cls):
     """The inference path (fused layer kernel, then the norm) and the training path with the
-    dropout off are the same model; a one-rank shard gives its rows."""
+    dropout off are the same model, and the CPU's."""
     g, adj = _graph()
     g = g.to(cuda)
     m = _model(cls, layer_norm=True).to(cuda).eval()
@@ -189,15 +189,27 @@ def test_ngcf_layer_norm_inference(cuda, cls):
         fast = torch.cat(m(g))
     slow = torch.cat(m(g)).detach()
     torch.testing.assert_close(fast, slow, rtol=1e-4, atol=1e-5)
-    from src.ops.distributed import DistributedGraph, ngcf_forward_dist
-    with torch.no_grad():
-        dg = DistributedGraph(g, 0, 1, cuda)
-        local = ngcf_forward_dist(dg, m, dg.pad_table(m._initial_table()))
-    assert torch.equal(local[:800], fast)
     cpu = _model(cls, layer_norm=True)
     cpu.load_state_dict({k: v.cpu() for k, v in m.state_dict().items()})
     with torch.no_grad():
         torch.testing.assert_close(fast.cpu(), torch.cat(cpu.eval()(adj)), rtol=1e-3, atol=1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [NGCF, NGCFGroupShuffle])
+def test_one_rank_shard_with_layer_norm(cuda, cls):
+    """A one-rank shard's native forward gives the rows of the model's own."""
+    from src.ops.distributed import DistributedGraph, ngcf_forward_dist
+    g, _ = _graph()
+    g = g.to(cuda)
+    dg = DistributedGraph(g, 0, 1, cuda)
+    with torch.no_grad():
+        m = _model(cls, sizes=(64, 64), layer_norm=True).to(cuda).eval()
+        local = ngcf_forward_dist(dg, m, dg.pad_table(m._initial_table()))
+        assert torch.equal(local[:800], torch.cat(m(g)))
+        m = _model(cls, layer_norm=True).to(cuda).eval()
+        with pytest.raises(NotImplementedError):     # a shard's layers keep their width
+            ngcf_forward_dist(dg, m, dg.pad_table(m._initial_table()))
 
 
 @pytest.mark.gpu
