@@ -8,8 +8,8 @@
 // E2M1 is the 4-bit type that this hardware converts by itself (two codes an instruction).
 //
 // All of it is bound by the table's bytes: one user against 1M x 64 9.6 us (4.2 TB/s), 16 users
-// against 1M x 256 bf16 48 us (3.7), 8192 x 8192 and one user 16 us (2.3: latency of two rounds of
-// loads); the quantiser 1M x 64 fp32 66 us (4.4).
+// against 1M x 256 bf16 48 us (3.7), 8192 x 8192 and one user 13.7 us (2.8: latency of
+// rounds of loads); the quantiser 1M x 64 fp32 66 us (4.4).
 #include <type_traits>
 
 #include "rowwise.h"
@@ -414,17 +414,20 @@ __global__ __launch_bounds__(WK * 64, 4) void q4_few_kernel(const T* __restrict_
   const int users = (int)(p.m - user0 < 4 ? p.m - user0 : 4);
   const int per = (int)p.ng * 4, pitch = per + 4;  // 16-B pieces
   const int64_t steps = (p.ng + 3) >> 2;
-  const int64_t b0 = steps * wave / WK, b1 = steps * (wave + 1) / WK;
+  // a wave's steps are wave, wave + WK, ...: the waves read neighbouring pieces of the rows
+  const int64_t count = (steps - wave + WK - 1) / WK;
   const int64_t tasks = (p.n + NT * 16 - 1) / (NT * 16);
   // rows of A that no user fills repeat another's: they reach no result that is stored
   const int mine = (min(r >> 2, kP - 1) * users + min(r & 3, users - 1)) * pitch + q;
   Codes<NT, 4> now[STEPS];
   auto load = [&](int64_t task, int64_t b) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i)
-      now[i].load(p, task * NT * 16, (b + i < steps ? b + i : steps - 1) * 4);
+    for (int i = 0; i < STEPS; ++i) {
+      const int64_t step = wave + (b + i) * WK;
+      now[i].load(p, task * NT * 16, (step < steps ? step : steps - 1) * 4);
+    }
   };
-  load(blockIdx.x, b0);
+  load(blockIdx.x, 0);
   for (int u = 0; u < users; ++u)
     for (int c = threadIdx.x; c < per; c += WK * 64) {
       float v[8];
@@ -437,20 +440,21 @@ __global__ __launch_bounds__(WK * 64, 4) void q4_few_kernel(const T* __restrict_
   __syncthreads();
   for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
     f32x4 acc[NT] = {};
-    if (task != blockIdx.x) load(task, b0);
-    for (int64_t b = b0;;) {
+    if (task != blockIdx.x) load(task, 0);
+    for (int64_t b = 0;;) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
-        if (b + i >= b1) break;
+        if (b + i >= count) break;
+        const int64_t g0 = (wave + (b + i) * WK) * 4;
         now[i].template multiply<1>(
-            p.ng - (b + i) * 4,
+            p.ng - g0,
             [&](int g, bf16x8(&f)[1]) {
-              f[0] = __builtin_bit_cast(bf16x8, rows[mine + ((b + i) * 4 + g) * 4]);
+              f[0] = __builtin_bit_cast(bf16x8, rows[mine + (g0 + g) * 4]);
             },
             acc);
       }
       b += STEPS;
-      if (b >= b1) break;
+      if (b >= count) break;
       load(task, b);
     }
     join_waves<NT, WK>(acc, join);
@@ -540,8 +544,13 @@ constexpr int64_t kWalkGrid = 768, kWalkGridTiled = 384, kSplitGrid = 1024;
 // with the joined sums the rows stay below 64 KB.
 constexpr int64_t kWalkBytes = 64 * 1024, kFewBytes = 50 * 1024;
 // Items from which waves walk long rows alone (125 000 x 512, one user: 13.1 us, split 49.3), and
-// from which a tile set is four tiles (4 users x 30 000 x 1 000: one tile 10.7 us, four 14.9).
+// from which they walk four tiles at a time (4 users x 30 000 x 1000: one tile 10.7 us, four
+// 14.9).
 constexpr int64_t kManyItems = 16384, kWideItems = 65536;
+// Items from which the waves that split long rows share two tiles (8192 x 8192, one user: 13.7 us,
+// one tile 15.6; 4096 x 4096: 8.4 and 6.5); eight waves from 2048 columns, four below (8000 x
+// 1000: 4.3 us, eight 4.9).
+constexpr int64_t kPairItems = 6144;
 
 static int64_t parts_of(int32_t dtype) {
   return dtype == GNNREC_F32 ? 3 : dtype == GNNREC_F16 ? 2 : 1;
@@ -596,28 +605,25 @@ static int run_few(int32_t dtype, const T* x, int64_t ldx, const Q4Args& p, hipS
   };
   using std::integral_constant;
   const integral_constant<int, 1> i1{};
-  const integral_constant<int, 4> i4{};
-  const integral_constant<int, 8> i8{};
-  if (p.n >= kManyItems) return go(i4, i4, i1);
-  return p.ng >= 128 ? go(i1, i8, i4) : go(i1, i4, i4);
-}
-
-template <int PARTS>
-static int run_many(const bf16_t* x, int64_t ldx, int64_t plane, const Q4Args& p,
-                    hipStream_t stream) {
-  auto go = [&](auto nt, auto wk) {
-    const int64_t tasks = ceil_div(p.n, nt.value * 16);
-    hipLaunchKernelGGL((q4_many_kernel<PARTS, nt.value, wk.value>),
-                       dim3((unsigned)(tasks < kSplitGrid ? tasks : kSplitGrid),
-                            (unsigned)ceil_div(p.m, 16)),
-                       dim3(wk.value * 64), 0, stream, x, ldx, plane, p);
-    return check_launch("q4_matmul");
-  };
-  using std::integral_constant;
   const integral_constant<int, 2> i2{};
   const integral_constant<int, 4> i4{};
   const integral_constant<int, 8> i8{};
-  return p.n >= kManyItems || p.ng < 128 ? go(i4, i4) : go(i2, i8);
+  if (p.n >= kPairItems) return p.ng >= 64 ? go(i2, i8, i2) : go(i2, i4, i2);
+  return p.ng >= 64 ? go(i1, i8, i2) : go(i1, i4, i2);
+}
+
+// Two tiles, four waves: 16 users x 8192 x 8192 fp32 35.3 us (eight waves 36.3), x 2000 x 1000 9.6
+// (four tiles 12.2), x 20 000 x 3100 bf16 20.2 (four tiles 22.4, eight waves 23.0).
+template <int PARTS>
+static int run_many(const bf16_t* x, int64_t ldx, int64_t plane, const Q4Args& p,
+                    hipStream_t stream) {
+  constexpr int kTiles = 2, kWaves = 4;
+  const int64_t tasks = ceil_div(p.n, kTiles * 16);
+  hipLaunchKernelGGL((q4_many_kernel<PARTS, kTiles, kWaves>),
+                     dim3((unsigned)(tasks < kSplitGrid ? tasks : kSplitGrid),
+                          (unsigned)ceil_div(p.m, 16)),
+                     dim3(kWaves * 64), 0, stream, x, ldx, plane, p);
+  return check_launch("q4_matmul");
 }
 
 static int check_table(const char* what, int64_t n, int64_t k, const void* codes,
