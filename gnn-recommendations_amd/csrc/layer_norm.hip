@@ -19,8 +19,9 @@
 // (no atomics: equal inputs give equal bits).
 //
 // fp32 tables are bound by memory (the block on 2M x 64: forward 187 us, 5.5 TB/s, backward 302 us,
-// 5.1, sums 6 us); half-precision blocks by instructions, most of them the generator's and the
-// conversions' (100 003 x 201 fp16: 38, 61 and 7 us, 62 % of the VALU's cycles busy forward).
+// 5.1, sums 4 us), wide half-precision rows too (8192 x 4096 bf16 alone: 30, 44 and 5 us);
+// half-precision blocks by instructions, most of them the generator's and the conversions' (100 003
+// x 201 fp16: 38, 60 and 4 us, the VALU busy in 64 and 62 % of the cycles).
 #include <type_traits>
 
 #include "rowwise.h"
