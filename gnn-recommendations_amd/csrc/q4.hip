@@ -278,7 +278,7 @@ struct Codes {
 
 // The results of NT tiles. Lane (q, r) holds users 4 q + i of item r of a tile, or part q of user
 // i; a transposition gives a register 64 neighbouring items of one user (NT == 4), or the parts
-// of user q (FEW, NT == 1).
+// of user q (FEW, fewer tiles).
 template <bool FEW, int NT, int PARTS>
 __device__ __forceinline__ void store_tiles(const Q4Args& p, int64_t base, int64_t user0,
                                             const f32x4 (&acc)[NT]) {
@@ -691,6 +691,7 @@ extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, con
   GNNREC_REQUIRE(gnnrec_q4_matmul_work_bytes(dtype, m, n, k) == 0 || (work && aligned16(work)),
                  "q4_matmul: the workspace is missing or not 16-B aligned");
   const int64_t ng = ceil_div(k, kGroup);
+  GNNREC_REQUIRE(ceil_div(m * ng * 4, kQ4Block) <= 0x7fffffff, "q4_matmul: x is too large");
   const Q4Args p{m, n, k, ng, ldo, (const uint32_t*)codes, (const bf16_t*)scale, out, out_dtype};
   const hipStream_t st = as_hip(stream);
   return with_dtype(dtype, [&](auto e) {

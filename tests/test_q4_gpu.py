@@ -88,13 +88,16 @@ def test_range_of_x(cuda):
     assert not ops.q4_matmul(torch.zeros(3, 96, device="cuda"), t).any()
 
 
-def test_non_finite_values(cuda):
-    """An infinity or a NaN of one user reaches that user's scores as in the full product."""
-    t = _table(80, 64, seed=3)
-    v = R.q4_values(t.codes, t.scale, 64)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [64, 300, 2080])
+def test_non_finite_values(cuda, dtype, k):
+    """An infinity or a NaN of one user reaches that user's scores as in the full product, in
+    each of the kernels (by the width and the number of users)."""
+    t = _table(80, k, seed=3)
+    v = R.q4_values(t.codes, t.scale, k)
     for m in (1, 2, 7, 20):
         for bad in (float("inf"), float("-inf"), float("nan")):
-            x = torch.randn(m, 64, generator=torch.Generator().manual_seed(1))
+            x = torch.randn(m, k, generator=torch.Generator().manual_seed(1)).to(dtype)
             clean = ops.q4_matmul(x.cuda(), t)
             x[m // 2, 40] = bad
             got = ops.q4_matmul(x.cuda(), t).cpu()
@@ -104,6 +107,10 @@ def test_non_finite_values(cuda):
             assert torch.equal(got[m // 2][inf].double(), want[inf])
             rest = torch.arange(m) != m // 2
             assert torch.equal(got[rest], clean.cpu()[rest])
+
+
+def test_nan_payloads_and_scales(cuda):
+    t = _table(80, 64, seed=3)
     # a NaN with only low payload bits, which half of a word would take for an infinity
     x = torch.zeros(1, 64)
     x.view(torch.int32)[0, 3] = 0x7F800001
