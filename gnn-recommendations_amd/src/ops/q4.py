@@ -102,8 +102,11 @@ def quantize_q4(w: torch.Tensor) -> Q4Table:
 def q4_matmul(x: torch.Tensor, table: Q4Table,
               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [m, k] (or [k]) times the table's rows: scores [m, n] (or [n]) in out_dtype (default
-    x's). The products are exact (a code times a scale is not rounded) and summed in fp32. x:
-    fp32 / bf16 / fp16 rows of any stride, at most 65535 of them."""
+    x's). The products are exact (a code times a scale is not rounded) and summed in fp32, a
+    group's before its scale is applied: values of x up to 2^110 cannot overflow there, and fp32
+    values keep all their bits down to 2^-110 (below that the matrix cores drop parts smaller
+    than 2^-126). x: fp32 / bf16 / fp16 rows of any stride, at most 65535 of them. The scores
+    carry no gradient."""
     if not isinstance(table, Q4Table):
         raise TypeError(f"q4_matmul: expected a Q4Table, got {type(table).__name__}")
     codes, k = table.codes, table.k

@@ -694,7 +694,8 @@ int gnnrec_dequantize_q4(int64_t n, int64_t k, const void* codes, const void* sc
 
 /* out[i, r] = sum_c x[i, c] * value[r, c]: scores of m <= 65535 users' rows (x: [m, k] of dtype)
  * against all n items of a 4-bit table, as user_emb @ item_emb.T (evaluator.py:96) does with
- * full-width items. The products are exact and summed in fp32; out is [m, n] of out_dtype.
+ * full-width items. The products are exact and summed in fp32 (a group's before its
+ * scale; |x| from 2^-110 to 2^110); out is [m, n] of out_dtype.
  * work: gnnrec_q4_matmul_work_bytes(dtype, m, n, k) bytes of scratch, 16-B aligned, that no call
  * running at the same time uses (often 0: then NULL). */
 int64_t gnnrec_q4_matmul_work_bytes(int32_t dtype, int64_t m, int64_t n, int64_t k);
