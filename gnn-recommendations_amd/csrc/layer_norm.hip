@@ -66,9 +66,9 @@ __device__ __forceinline__ float moved(float v) {
 template <int L>
 __device__ __forceinline__ void lane_sum2(float& a, float& b) {
   auto step = [&](float x, float y) { a += x, b += y; };
-  step(moved<0xB1>(a), moved<0xB1>(b));                // quad_perm 1 0 3 2
-  step(moved<0x4E>(a), moved<0x4E>(b));                // quad_perm 2 3 0 1
-  step(moved<0x141>(a), moved<0x141>(b));              // mirror within 8
+  if (L >= 2) step(moved<0xB1>(a), moved<0xB1>(b));    // quad_perm 1 0 3 2
+  if (L >= 4) step(moved<0x4E>(a), moved<0x4E>(b));    // quad_perm 2 3 0 1
+  if (L >= 8) step(moved<0x141>(a), moved<0x141>(b));  // mirror within 8
   if (L >= 16) step(moved<0x140>(a), moved<0x140>(b));  // mirror within 16
   if (L >= 32) {
     const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
@@ -387,11 +387,22 @@ __global__ __launch_bounds__(TPR > kNormBlock ? TPR : kNormBlock,
       for (int e = 0; e < 8; ++e)
         join[threadIdx.x * 8 + e] = k ? ab[LATE ? 0 : j][e] : aw[LATE ? 0 : j][e];
       __syncthreads();
-      for (int i = threadIdx.x; i < TPR * 8; i += kBlock) {
-        const int64_t c = (int64_t)j * TPR * 8 + i;
+      constexpr int kCols = TPR * 8, kSlices = kBlock / kCols;
+      if (kSlices > 1) {  // few columns: eight groups a thread, then the threads of a column
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          s += join[(threadIdx.x / kCols * 8 + q) * kCols + threadIdx.x % kCols];
+        __syncthreads();
+        join[threadIdx.x] = s;
+        __syncthreads();
+      }
+      constexpr int kLeft = kSlices > 1 ? kSlices : kGroups;
+      for (int i = threadIdx.x; i < kCols; i += kBlock) {
+        const int64_t c = (int64_t)j * kCols + i;
         if (c >= in.d) continue;
         float s = 0.f;
-        for (int q = 0; q < kGroups; ++q) s += join[q * TPR * 8 + i];
+        for (int q = 0; q < kLeft; ++q) s += join[q * kCols + i];
         part[(int64_t)blockIdx.x * 2 * in.d + k * in.d + c] = s;
       }
     }
@@ -429,10 +440,11 @@ __global__ __launch_bounds__(kSumBlock) void norm_sum_kernel(const float* __rest
   }
 }
 
-// Lanes a row and blocks a lane by the row's width (blocks of eight columns): one wave holds up
-// to 1024 columns, wider rows take a workgroup. Rows that fill every lane (a power of two from 64
-// columns on) have an instance without masks, and rows of a workgroup one for the norm alone,
-// without registers for a residual and a mask.
+// Lanes a row and blocks a lane by the row's width (blocks of eight columns), from one lane on (1M
+// x 16 fp16 block: two lanes a row 66 us, eight 166; 1M x 32 bf16: four 125, eight 182): one wave
+// holds up to 1024 columns, wider rows take a workgroup. Rows that fill every lane (a power of two
+// from 16 columns on) have an instance without masks, and rows of a workgroup one for the norm
+// alone, without registers for a residual and a mask.
 template <int TPR, int NV, Edge EDGE, bool PLAIN>
 struct Shape {
   static constexpr int tpr = TPR, nv = NV;
@@ -452,7 +464,9 @@ static int workgroup(int64_t d, bool plain, F&& f) {
 template <class F>
 static int with_shape(int64_t d, bool plain, F&& f) {
   const int64_t nb = ceil_div(d, 8);
-  if (d < 8) return f(Shape<8, 1, kNarrow, false>{});
+  if (d < 8) return f(Shape<1, 1, kNarrow, false>{});
+  if (nb <= 2) return one_wave<2, 1>(d, f);
+  if (nb <= 4) return one_wave<4, 1>(d, f);
   if (nb <= 8) return one_wave<8, 1>(d, f);
   if (nb <= 16) return one_wave<16, 1>(d, f);
   if (nb <= 32) return one_wave<32, 1>(d, f);

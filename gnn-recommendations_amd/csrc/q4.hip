@@ -612,18 +612,24 @@ static int run_few(int32_t dtype, const T* x, int64_t ldx, const Q4Args& p, hipS
   return p.ng >= 64 ? go(i1, i8, i2) : go(i1, i4, i2);
 }
 
-// Two tiles, four waves: 16 users x 8192 x 8192 fp32 35.3 us (eight waves 36.3), x 2000 x 1000 9.6
-// (four tiles 12.2), x 20 000 x 3100 bf16 20.2 (four tiles 22.4, eight waves 23.0).
+// Two tiles a wave set: 16 users x 8192 x 8192 fp32 35.3 us (eight waves 36.3), x 2000 x 1000 9.6
+// (four tiles 12.2), x 20 000 x 3100 bf16 20.2 (four tiles 22.4). Four where there are several
+// user tiles and many items, so that a fragment serves more of them: 64 users x 7812 x 8192 82 us
+// (two 120), x 10 000 x 1000 23.4 (25.6); but x 300 x 3000 22.2 (17.3).
 template <int PARTS>
 static int run_many(const bf16_t* x, int64_t ldx, int64_t plane, const Q4Args& p,
                     hipStream_t stream) {
-  constexpr int kTiles = 2, kWaves = 4;
-  const int64_t tasks = ceil_div(p.n, kTiles * 16);
-  hipLaunchKernelGGL((q4_many_kernel<PARTS, kTiles, kWaves>),
-                     dim3((unsigned)(tasks < kSplitGrid ? tasks : kSplitGrid),
-                          (unsigned)ceil_div(p.m, 16)),
-                     dim3(kWaves * 64), 0, stream, x, ldx, plane, p);
-  return check_launch("q4_matmul");
+  auto go = [&](auto nt) {
+    constexpr int kWaves = 4;
+    const int64_t tasks = ceil_div(p.n, nt.value * 16);
+    hipLaunchKernelGGL((q4_many_kernel<PARTS, nt.value, kWaves>),
+                       dim3((unsigned)(tasks < kSplitGrid ? tasks : kSplitGrid),
+                            (unsigned)ceil_div(p.m, 16)),
+                       dim3(kWaves * 64), 0, stream, x, ldx, plane, p);
+    return check_launch("q4_matmul");
+  };
+  if (p.m > 16 && p.n >= kPairItems) return go(std::integral_constant<int, 4>{});
+  return go(std::integral_constant<int, 2>{});
 }
 
 static int check_table(const char* what, int64_t n, int64_t k, const void* codes,
