@@ -157,7 +157,7 @@ def _check_block(rows, d, dtype, wdtype, p, slope, with_res, with_w, shift=0.0, 
         R.assert_close(v, *want[name], f"{name} {rows}x{d} {dtype}")
 
 
-WIDTHS = [1, 2, 3, 7, 8, 9, 31, 64, 65, 100, 128, 129, 255, 256, 321, 512, 513, 1000, 1024, 1025,
+WIDTHS = [1, 2, 3, 7, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 128, 129, 255, 256, 321, 512, 513, 1000, 1024, 1025,
           2048, 2049, 4096, 4097, 8192, 8193, 16384]
 
 
@@ -190,6 +190,14 @@ def test_block_variants(cuda, with_res, with_w, p, slope):
 @pytest.mark.parametrize("rows", [1, 2, 31, 33, 1025, 5000, 40000])
 def test_rows(cuda, rows):
     _check_block(rows, 40, F32, F32, 0.1, 0.2, True, True)
+
+
+@pytest.mark.parametrize("d", [3, 8, 16, 30, 32])
+@pytest.mark.parametrize("rows", [300, 5001, 70000])
+def test_rows_of_few_values(cuda, rows, d):
+    """Rows of one to four lanes: up to 256 of them in a workgroup's sums."""
+    _check_block(rows, d, F32, F32, 0.1, 0.2, True, True)
+    _check_block(rows, d, BF16, F32, 0.0, 1.0, False, True)
 
 
 def test_far_mean_and_constant_rows(cuda):
