@@ -27,17 +27,12 @@ TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)     # E2M1, by the low three bits
 
 
-_OPS = None
-
-
 def _ops():
-    """The framework's operators, imported once, as a program does."""
-    global _OPS
-    if _OPS is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "gnn-recommendations_amd"))
-        from src import ops
-        _OPS = ops
-    return _OPS
+    root = Path(__file__).resolve().parents[1] / "gnn-recommendations_amd"
+    if str(root) not in sys.path:
+        sys.path.insert(0, str(root))
+    from src import ops
+    return ops
 
 
 # ---- the cases ---------------------------------------------------------------------------
