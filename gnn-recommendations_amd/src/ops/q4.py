@@ -7,7 +7,7 @@ A Q4Table holds E2M1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), two 
 even column in the low half, rows padded to whole groups of 32 columns, and one bfloat16 scale
 for each group of a row. One user's scores read the table once, so they take the time of its
 bytes: an eighth of an fp32 table's, and a catalogue that fits the caches eight times later.
-Serving only: the scores carry no gradient.
+Serving only: the scores carry no gradient and no forward-mode tangent, whatever x does.
 """
 from __future__ import annotations
 

@@ -8,9 +8,9 @@ generator, layer norm, and the block between two hops that joins them.
 
 Tables on a ROCm device, fp32 / bf16 / fp16, 2-D row-major views with any row stride (0 too) or
 contiguous tensors of any rank (rows are the last dimension); launched on torch's current stream
-of the table's device. All differentiable (once), each backward pass one launch (two with a
-weight gradient) that repeats the forward's arithmetic from its inputs: no mask, statistics or
-normalised rows are kept.
+of the table's device. All differentiable (once, in reverse: a forward-mode tangent raises),
+each backward pass one launch (two with a weight gradient) that repeats the forward's arithmetic
+from its inputs: no mask, statistics or normalised rows are kept.
 
 The dropout's mask: value (row, column) is dropped when its 16-bit draw is below
 round(p * 65536), the others are scaled by 65536 / (65536 - round(p * 65536)). The draws are
@@ -30,6 +30,7 @@ from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -139,15 +140,23 @@ _NO_MASK = (None, (0.0, 0), (0, 0, 1.0))
 
 
 def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether autograd records a call with these inputs (otherwise its bookkeeping is skipped)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether autograd has to see a call with these inputs (otherwise its bookkeeping is
+    skipped): one is recorded, or a forward-mode level is open. There an input may carry a
+    tangent, whether it requires a gradient or not, and autograd refuses it (no jvp)."""
+    return (forward_ad._current_level >= 0
+            or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def _once(backward):
-    """once_differentiable(backward), without its cost where no second derivative is asked for."""
+    """once_differentiable(backward), without its cost where no second derivative is asked for.
+    A gradient with a forward-mode tangent is refused: the launch would lose it."""
     guarded = once_differentiable(backward)
 
     def wrapped(ctx, *grads):
+        if forward_ad._current_level >= 0:
+            if any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+                raise NotImplementedError("the row-wise operators' backward passes have no "
+                                          "forward-mode derivative")
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
     return staticmethod(wrapped)
 
