@@ -21,6 +21,9 @@ is an int or a one-element int64 tensor on the table's device; a captured graph 
 on every replay, so `seed.add_(1)` between replays (or captured in front) gives new masks.
 A dropped value is 0 whatever x holds there, also an infinity or a NaN.
 
+Nothing here can be traced into a graph of torch operators (torch.jit.trace, make_fx,
+torch.export raise); under torch.compile a call runs between the compiled parts.
+
 Forward and backward may be captured into a graph. As for any torch operator, no eager autograd
 graph of the same leaves may be alive while a backward pass is captured.
 """
@@ -34,7 +37,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, ptr
+from ._lib import check
 
 MAX_NORM_WIDTH = 16384    # csrc/layer_norm.hip kNormMaxD
 
@@ -48,9 +51,25 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
+_jit_tracing = torch._C._get_tracing_state
+_modes = torch._C._len_torch_dispatch_stack
+_pre_dispatch_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
+
+
+def _refuse_tracing(name: str) -> None:
+    """Raise if a graph is being recorded (and not if another dispatch mode is active)."""
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    if _jit_tracing() is not None or get_proxy_mode() is not None:
+        raise RuntimeError(f"{name}: cannot be traced; a recorded graph would hold the result's "
+                           "allocation without the launch that fills it, and this call's sizes")
+
+
 def launch(name: str, device: torch.device, *args) -> None:
-    """Call a C entry on `device`'s current stream, whatever device is current. The calls of a
-    small table cost the host more than the GPU, so nothing is looked up twice here."""
+    """Call a C entry on `device`'s current stream, whatever device is current; refused while
+    torch.jit.trace or make_fx records. The calls of a small table cost the host more than the
+    GPU, so nothing is looked up twice here."""
+    if _jit_tracing() is not None or _modes() or _pre_dispatch_modes():
+        _refuse_tracing(name)
     fn = _ENTRIES.get(name)
     if fn is None:
         fn = _ENTRIES[name] = getattr(_lib.lib(), name)
@@ -62,6 +81,18 @@ def launch(name: str, device: torch.device, *args) -> None:
             rc = fn(*args, _raw_stream(i))
     if rc:
         check(rc, name)
+
+
+def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    """t's address, None for no tensor. One without memory of its own (functionalize's wrappers)
+    is refused: its address reads as NULL, which to a C entry is an absent table."""
+    if t is None:
+        return None
+    address = t.data_ptr()
+    if not address and t.numel():
+        raise RuntimeError(f"the row-wise operators need tensors in memory, got {type(t).__name__} "
+                           f"{tuple(t.shape)} without an address")
+    return address
 
 
 def rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -165,8 +196,8 @@ def _dropout_forward(x, ldx, rows, mask):
     seed_t, pre, post = mask
     y = _empty_rows(x)
     d = x.shape[-1]
-    launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, x.data_ptr(), ldx,
-           y.data_ptr(), d, *pre, ptr(seed_t), *post)
+    launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, ptr(x), ldx,
+           ptr(y), d, *pre, ptr(seed_t), *post)
     return y
 
 
@@ -188,7 +219,7 @@ class _Dropout(torch.autograd.Function):
         dx = _empty_rows(dy)
         d = dy.shape[-1]
         launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x), ldx,
-               dy.data_ptr(), lddy, dx.data_ptr(), d, *pre, ptr(seed_t), *post)
+               ptr(dy), lddy, ptr(dx), d, *pre, ptr(seed_t), *post)
         return dx, None, None, None
 
 
@@ -210,8 +241,8 @@ def _norm_forward(x, res, w, b, cfg):
     y = _empty_rows(x)
     h = torch.empty_like(y) if keep_h else None
     d = x.shape[-1]
-    launch("gnnrec_layer_norm_forward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res), ldr,
-           ptr(w), ptr(b), eps, *pre, ptr(seed_t), *post, y.data_ptr(), d, ptr(h), d)
+    launch("gnnrec_layer_norm_forward", x.device, t, wt, rows, d, ptr(x), ldx, ptr(res), ldr,
+           ptr(w), ptr(b), eps, *pre, ptr(seed_t), *post, ptr(y), d, ptr(h), d)
     return y, h
 
 
@@ -245,8 +276,8 @@ class _NormBlock(torch.autograd.Function):
         work = None
         if need_w or need_b:
             work = x.new_empty(_norm_work_floats(rows, d), dtype=torch.float32)
-        launch("gnnrec_layer_norm_backward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res),
-               ldr, ptr(w), eps, *pre, ptr(seed_t), *post, dy.data_ptr(), lddy, ptr(dh), lddh,
+        launch("gnnrec_layer_norm_backward", x.device, t, wt, rows, d, ptr(x), ldx, ptr(res),
+               ldr, ptr(w), eps, *pre, ptr(seed_t), *post, ptr(dy), lddy, ptr(dh), lddh,
                ptr(dx), d, ptr(dres), d, ptr(dw), ptr(db), ptr(work))
         return dx, dres, dw, db, None
 

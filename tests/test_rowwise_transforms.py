@@ -1,12 +1,15 @@
 """The row-wise operators under torch's transforms: an input with a forward-mode tangent is
-refused, since the operators have no such derivative. Without a GPU the C entries are stood in
-for; the same calls run on the device below."""
+refused, since the operators have no such derivative, and so is every tracer, which would record
+the result's allocation alone. Without a GPU the C entries are stood in for; the same calls run
+on the device below."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
 
 from src import ops
-from src.ops import rowwise
+from src.ops import q4, rowwise
 
 
 @pytest.fixture
@@ -20,6 +23,7 @@ def stand_in(monkeypatch):
     monkeypatch.setattr(rowwise, "_current_device", lambda: None)
     monkeypatch.setattr(rowwise, "_raw_stream", lambda i: 0)
     monkeypatch.setattr(rowwise, "rows_of", lambda t, what: t.view(-1, t.shape[-1]))
+    monkeypatch.setattr(q4, "rows_of", rowwise.rows_of)
     return torch.device("cpu")
 
 
@@ -66,3 +70,44 @@ def test_tangents_of_other_inputs_are_refused(stand_in):
 @pytest.mark.parametrize("call", CALLS)
 def test_tangents_are_refused_on_the_device(cuda, call):
     _tangents(cuda, CALLS[call])
+
+
+def _traces(device, call):
+    for leaf in (False, True):
+        x = torch.ones(4, 8, device=device, requires_grad=leaf)
+        for tracer in (lambda: torch.jit.trace(call, (x,), check_trace=False),
+                       lambda: make_fx(call)(x), lambda: make_fx(call, pre_dispatch=True)(x),
+                       lambda: make_fx(call, tracing_mode="fake")(x),
+                       lambda: torch.func.functionalize(call)(x)):
+            with pytest.raises((RuntimeError, ValueError)):
+                tracer()
+        y = call(x)
+        if leaf and y.requires_grad:           # the backward pass alone
+            with pytest.raises(RuntimeError, match="traced"):
+                make_fx(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0])(y.detach())
+        with FlopCounterMode(display=False):   # a mode that records no graph is none of this
+            assert call(x).shape == y.shape
+
+
+def _table(device):
+    return ops.Q4Table(torch.zeros(3, 16, dtype=torch.uint8, device=device),
+                       torch.ones(3, 1, device=device).bfloat16(), 8)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("call", [*CALLS, "q4_matmul", "quantize_q4"])
+def test_tracing_is_refused(stand_in, call):
+    table = _table(stand_in)
+    _traces(stand_in, {"q4_matmul": lambda x: ops.q4_matmul(x, table),
+                       "quantize_q4": lambda x: ops.quantize_q4(x).scale}.get(call)
+            or CALLS[call])
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("call", [*CALLS, "q4_matmul", "quantize_q4", "dequantize"])
+def test_tracing_is_refused_on_the_device(cuda, call):
+    table = _table(cuda)
+    _traces(cuda, {"q4_matmul": lambda x: ops.q4_matmul(x, table),
+                   "quantize_q4": lambda x: ops.quantize_q4(x).scale,
+                   "dequantize": lambda x: table.dequantize() + x.detach()[:3]}.get(call) or CALLS[call])
