@@ -201,6 +201,17 @@ def _dropout_forward(x, ldx, rows, mask):
     return y
 
 
+def _dropout_backward(x, dy, rows, mask):
+    seed_t, pre, post = mask
+    x, ldx = _dense_rows(x)
+    dy, lddy = _dense_rows(dy)
+    dx = _empty_rows(dy)
+    d = dy.shape[-1]
+    launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x), ldx,
+           ptr(dy), lddy, ptr(dx), d, *pre, ptr(seed_t), *post)
+    return dx
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ldx, rows, mask):
@@ -214,13 +225,7 @@ class _Dropout(torch.autograd.Function):
     def backward(ctx, dy):
         x, seed_t = ctx.saved_tensors
         rows, pre, post = ctx.cfg
-        x, ldx = _dense_rows(x)
-        dy, lddy = _dense_rows(dy)
-        dx = _empty_rows(dy)
-        d = dy.shape[-1]
-        launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x), ldx,
-               ptr(dy), lddy, ptr(dx), d, *pre, ptr(seed_t), *post)
-        return dx, None, None, None
+        return _dropout_backward(x, dy, rows, (seed_t, pre, post)), None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: Seed, *, site: int = 0, row0: int = 0,
@@ -262,8 +267,12 @@ class _NormBlock(torch.autograd.Function):
         need_x, need_r, need_w, need_b, _ = ctx.needs_input_grad
         if dy is None and dh is None:
             return None, None, None, None, None
-        if dy is None:      # only h was used: nothing passes through the norm
-            dy = torch.zeros_like(dh)
+        if dy is None:
+            # only h was used: nothing passes through the norm, which a row may not have (a NaN
+            # in it, a constant one without eps)
+            dx = _dropout_backward(x, dh, rows, (seed_t, pre, post)) if need_x else None
+            return (dx, dh if need_r else None, torch.zeros_like(w) if need_w else None,
+                    x.new_zeros(x.shape[-1], dtype=ctx.b_dtype) if need_b else None, None)
         x, ldx = _dense_rows(x)
         res, ldr = _dense_rows(res)
         dy, lddy = _dense_rows(dy)
