@@ -21,7 +21,7 @@ __global__ __launch_bounds__(kDropBlock) void dropout_kernel(
     int64_t rows, int64_t d, int64_t nb, const T* __restrict__ x, int64_t ldx,
     const T* __restrict__ dy, int64_t lddy, T* __restrict__ out, int64_t ldo, Drop drop) {
   // items (row, block of eight columns) in row order; the 64-bit division is the block's own
-  const int64_t base = (int64_t)blockIdx.x * kDropBlock;
+  const int64_t base = block_index() * kDropBlock;
   const int64_t row_base = base / nb;
   const uint32_t in_row = (uint32_t)(base - row_base * nb) + threadIdx.x;
   const uint32_t q = in_row / (uint32_t)nb, cb = in_row - q * (uint32_t)nb;
@@ -77,8 +77,9 @@ static int run_dropout(const char* what, int32_t dtype, int64_t rows, int64_t d,
     auto* kernel = d < 8        ? dropout_kernel<T, BWD, kNarrow>
                    : d % 8 == 0 ? dropout_kernel<T, BWD, kFull>
                                 : dropout_kernel<T, BWD, kRagged>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kDropBlock), 0, as_hip(stream), rows,
-                       d, nb, (const T*)x, ldx, (const T*)dy, lddy, (T*)out, ldo, drop);
+    hipLaunchKernelGGL(kernel, wide_grid(blocks, kDropBlock), dim3(kDropBlock), 0,
+                       as_hip(stream), rows, d, nb, (const T*)x, ldx, (const T*)dy, lddy, (T*)out,
+                       ldo, drop);
     return check_launch(what);
   });
 }

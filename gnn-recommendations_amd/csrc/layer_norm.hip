@@ -545,7 +545,8 @@ extern "C" int gnnrec_layer_norm_forward(int32_t dtype, int32_t wdtype, int64_t 
       // once (100 003 x 201 fp16 block, both passes: 118 -> 110 us); the others by memory, and
       // one row a lane group keeps more of it in flight (2M x 64 fp32: 960 us, resident 1000)
       const int64_t want = ceil_div(rows, kBlock / S::tpr);
-      const int64_t most = sizeof(T) == 2 && !S::plain ? 2048 : 0x7fffffff;
+      // (a grid has fewer than 2^32 threads; its workgroups take the rows beyond in turn)
+      const int64_t most = sizeof(T) == 2 && !S::plain ? 2048 : 0xffffffffll / kBlock;
       hipLaunchKernelGGL((norm_forward_kernel<T, S::tpr, S::nv, S::edge, S::plain>),
                          dim3((unsigned)(want < most ? want : most)),
                          dim3(kBlock), 0, as_hip(stream), in, (T*)y, ldy, (T*)h, ldh);

@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kQ4Block) void quantize_q4_kernel(int64_t n, int64_
                                                                int64_t ldw,
                                                                uint32_t* __restrict__ codes,
                                                                bf16_t* __restrict__ scale) {
-  const int64_t base = (int64_t)blockIdx.x * kQ4Block;
+  const int64_t base = block_index() * kQ4Block;
   const int64_t per_row = ng * 4;
   const int64_t row_base = base / per_row;
   const uint32_t in_row = (uint32_t)(base - row_base * per_row) + threadIdx.x;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kQ4Block) void dequantize_q4_kernel(int64_t n, int6
                                                                  const bf16_t* __restrict__ scale,
                                                                  float* __restrict__ out,
                                                                  int64_t ldo) {
-  const int64_t base = (int64_t)blockIdx.x * kQ4Block;
+  const int64_t base = block_index() * kQ4Block;
   const int64_t per_row = ng * 4;
   const int64_t row_base = base / per_row;
   const uint32_t in_row = (uint32_t)(base - row_base * per_row) + threadIdx.x;
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(kQ4Block) void split_users_kernel(const T* __restri
                                                                int64_t kp,
                                                                bf16_t* __restrict__ parts) {
   constexpr int kP = Parts<T>::n;
-  const int64_t i = (int64_t)blockIdx.x * kQ4Block + threadIdx.x;
+  const int64_t i = block_index() * kQ4Block + threadIdx.x;
   const int64_t per = kp / 8, row = i / per, c = (i - row * per) * 8;
   if (row >= m) return;
   float v[8];
@@ -656,7 +656,7 @@ extern "C" int gnnrec_quantize_q4(int32_t dtype, int64_t n, int64_t k, const voi
   const int64_t ng = ceil_div(k, kGroup);
   return with_dtype(dtype, [&](auto e) {
     using T = decltype(e);
-    hipLaunchKernelGGL((quantize_q4_kernel<T>), dim3((unsigned)ceil_div(n * ng * 4, kQ4Block)),
+    hipLaunchKernelGGL((quantize_q4_kernel<T>), wide_grid(ceil_div(n * ng * 4, kQ4Block), kQ4Block),
                        dim3(kQ4Block), 0, as_hip(stream), n, k, ng, (const T*)w, ldw,
                        (uint32_t*)codes, (bf16_t*)scale);
     return check_launch("quantize_q4");
@@ -669,7 +669,7 @@ extern "C" int gnnrec_dequantize_q4(int64_t n, int64_t k, const void* codes, con
   if (rc != GNNREC_OK || n == 0) return rc;
   GNNREC_REQUIRE(out, "dequantize_q4: null pointer");
   const int64_t ng = ceil_div(k, kGroup);
-  hipLaunchKernelGGL(dequantize_q4_kernel, dim3((unsigned)ceil_div(n * ng * 4, kQ4Block)),
+  hipLaunchKernelGGL(dequantize_q4_kernel, wide_grid(ceil_div(n * ng * 4, kQ4Block), kQ4Block),
                      dim3(kQ4Block), 0, as_hip(stream), n, k, ng, (const uint32_t*)codes,
                      (const bf16_t*)scale, out, ldo);
   return check_launch("dequantize_q4");
@@ -713,8 +713,8 @@ extern "C" int gnnrec_q4_matmul(int32_t dtype, int32_t out_dtype, int64_t m, con
     if (kP > 1 || k % kGroup) {
       const int64_t kp = ng * kGroup;
       hipLaunchKernelGGL((split_users_kernel<T>),
-                         dim3((unsigned)ceil_div(m * (kp / 8), kQ4Block)), dim3(kQ4Block), 0, st,
-                         (const T*)x, ldx, m, k, kp, (bf16_t*)work);
+                         wide_grid(ceil_div(m * (kp / 8), kQ4Block), kQ4Block), dim3(kQ4Block), 0,
+                         st, (const T*)x, ldx, m, k, kp, (bf16_t*)work);
       const int rc2 = check_launch("q4_matmul (users)");
       if (rc2 != GNNREC_OK) return rc2;
       xs = (const bf16_t*)work, lds = kp, plane = m * kp;

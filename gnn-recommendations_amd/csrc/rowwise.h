@@ -20,6 +20,17 @@ inline int with_dtype(int32_t t, F&& f) {
 }
 inline bool dtype_ok(int32_t t) { return t == GNNREC_F32 || t == GNNREC_BF16 || t == GNNREC_F16; }
 
+// The grid of a kernel whose workgroups (of `block` threads) are numbered by block_index(), with
+// at least `blocks` of them: HIP takes fewer than 2^32 threads in a dimension, and a table of 2^35
+// values has more eights than that, so the workgroups beyond go to further rows of the grid.
+inline dim3 wide_grid(int64_t blocks, int block) {
+  const int64_t rows = ceil_div(blocks, 0xffffffffll / block);
+  return dim3((unsigned)ceil_div(blocks, rows), (unsigned)rows);
+}
+__device__ __forceinline__ int64_t block_index() {
+  return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+}
+
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
