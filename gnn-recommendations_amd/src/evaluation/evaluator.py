@@ -169,6 +169,7 @@ class Evaluator:
             else:
                 if table is not None:
                     sc = q4_matmul(user_emb[b], table, out_dtype=torch.float32)
+                    sc.masked_fill_(sc.isnan(), float("-inf"))    # rank last, as score_topk's
                     at = np.repeat(np.arange(len(b)), counts)
                     sc[torch.from_numpy(at).to(sc.device),
                        torch.from_numpy(sub_col.astype(np.int64)).to(sc.device)] = float("-inf")
