@@ -179,6 +179,8 @@ class Evaluator:
                         sc[r, torch.from_numpy(sub_col[sub_ptr[r]:sub_ptr[r + 1]].astype(np.int64))] = float("-inf")
                 order = torch.sort(sc, dim=1, descending=True, stable=True).indices
                 idx = order[:, :k]
+                if table is not None and idx.shape[1] < k:    # -1 behind the last item, as there
+                    idx = torch.nn.functional.pad(idx, (0, k - idx.shape[1]), value=-1)
             rows.append(idx.cpu())
         return torch.cat(rows)
 

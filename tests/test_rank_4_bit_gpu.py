@@ -35,3 +35,11 @@ def test_items_without_a_score_rank_last(cuda):
     assert torch.equal(full, four)
     for r in four:
         assert 7 not in r.tolist() and 40 not in r.tolist()
+
+
+def test_more_places_than_items(cuda):
+    """Places that no item fills hold -1, as in the fp32 ranking."""
+    users, items = _exact_items(12, cuda)
+    full, four = _both(cuda, users, items, 20, [[3, 5], [], [11]])
+    assert four.shape == (3, 20) and torch.equal(full, four)
+    assert (four[:, 12:] == -1).all()
