@@ -113,6 +113,10 @@ def main(argv=None) -> int:
     if a.quick:
         a.seeds = a.seeds[:1]
     device = torch.device(a.device)
+    try:
+        evaluator = Evaluator(device=device, item_bits=a.item_bits)
+    except ValueError as e:    # before any model is trained
+        ap.error(str(e))
     if not a.skip_check:
         check_device(device)
     cfg = yaml.safe_load((ROOT / "config" / "training.yaml").read_text())
@@ -121,7 +125,8 @@ def main(argv=None) -> int:
     for ds_name in a.datasets:
         for model_name in a.models:
             for seed in a.seeds:
-                rec = {"model": model_name, "dataset": ds_name, "seed": seed, "status": "failed"}
+                rec = {"model": model_name, "dataset": ds_name, "seed": seed, "status": "failed",
+                       "item_bits": a.item_bits}
                 try:
                     torch.manual_seed(seed)
                     ds = load_dataset(ds_name, seed)
@@ -131,8 +136,7 @@ def main(argv=None) -> int:
                     adj = ds.get_graph(device) if device.type == "cuda" else ds.get_torch_adjacency()
                     rec["training_time"] = train_bpr(model, ds, adj, cfg, epochs, device, seed)
                     t0 = time.time()
-                    rec["test_metrics"] = Evaluator(
-                        device=device, item_bits=a.item_bits).evaluate(model, ds, adj_matrix=adj)
+                    rec["test_metrics"] = evaluator.evaluate(model, ds, adj_matrix=adj)
                     rec["eval_time"] = time.time() - t0
                     rec.update(status="success", n_users=ds.n_users, n_items=ds.n_items,
                                n_train=len(ds.train_data), epochs=epochs)
