@@ -53,7 +53,9 @@ class NGCFLayer(nn.Module):
     def normalised(self, z: torch.Tensor, x: torch.Tensor, p: float = 0.0, seed=0,
                    site: int = 0, negative_slope: float = 1.0) -> torch.Tensor:
         """LayerNorm(x + Dropout_p(LeakyReLU(z))); the layer's rows only, so a row shard may
-        call it with its own."""
+        call it with its own. Under autocast z is in half precision: the sum and the norm are in
+        x's fp32, which the next hop gathers."""
+        z = z.to(torch.promote_types(z.dtype, x.dtype))
         res = x if x.shape == z.shape else None
         if z.is_cuda:
             return ops.dropout_add_layer_norm(z, res, self.norm.weight, self.norm.bias, p, seed,
