@@ -84,7 +84,7 @@ class NGCFLayer(nn.Module):
             out = lin(n, self.W1) + lin(x * n, self.W2)
         else:
             out = self.W1(n) + self.W2(x * n)
-        p = self.dropout.p if self.training else 0.0
+        p = self.dropout.p if self.dropout.training else 0.0
         slope = self.activation.negative_slope
         if p > 0 and out.is_cuda and seed is None and (self.counter_dropout
                                                        or self.norm is not None):
@@ -131,8 +131,8 @@ class NGCF(BaseRecommender):
 
     def _mask_seed(self):
         """The seed of one training forward's counter-based masks, None where none is drawn."""
-        if not self.training or self.dropout == 0.0 or not any(
-                layer.counter_dropout or layer.norm is not None for layer in self.layers):
+        if not any(layer.dropout.training and layer.dropout.p > 0
+                   and (layer.counter_dropout or layer.norm is not None) for layer in self.layers):
             return None
         if self.dropout_seed is not None:
             return self.dropout_seed

@@ -34,3 +34,32 @@ def test_layer_norm_under_autocast(cuda, dtype):
         x = torch.cat(m(g))
     x.sum().backward()
     assert x.dtype == torch.float32 and torch.isfinite(m.user_embedding.weight.grad).all()
+
+
+@pytest.mark.parametrize("kw", [dict(counter_dropout=True), dict(layer_norm=True)])
+def test_masks_are_drawn_where_a_layer_drops(cuda, kw):
+    """A layer decides by its own mode and rate whether it drops: one that was switched after the
+    model was built, or alone (dropout at inference), draws like torch's dropout does."""
+    g, _ = _graph()
+    g = g.to(cuda)
+    m = _model(**kw).to(cuda).eval()
+    still = torch.cat(m(g)).detach()
+    assert torch.equal(still, torch.cat(m(g)))
+    m.layers[1].train()
+    torch.manual_seed(1)
+    one = torch.cat(m(g)).detach()
+    assert torch.equal(one[:, :128], still[:, :128]) and not torch.equal(one, still)
+    torch.manual_seed(1)
+    with torch.no_grad():
+        torch.testing.assert_close(torch.cat(m(g)), one, rtol=1e-4, atol=1e-5)
+    m.eval()
+    m.layers[1].dropout.train()                  # the dropout alone
+    torch.manual_seed(1)
+    assert torch.equal(torch.cat(m(g)), one)
+    m.train()
+    for layer in m.layers:
+        layer.dropout.p = 0.0
+    assert torch.equal(torch.cat(m(g)), torch.cat(m(g)))
+    m.layers[0].dropout.p = 0.5
+    m.dropout = 0.0
+    assert not torch.equal(torch.cat(m(g)), torch.cat(m(g)))
