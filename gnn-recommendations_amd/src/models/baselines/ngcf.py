@@ -15,8 +15,8 @@ Two options that the reference does not have, off by default:
   residual x where the widths differ), one native pass each way (ops.dropout_add_layer_norm),
   the mask counter-based as well. It keeps stacked hops from drifting to one direction and scale.
 Their masks' seed is drawn from torch's generator for every training forward, or read from
-``model.dropout_seed`` where that is set (a one-element int64 tensor on the device, so that a
-captured training step draws new masks on replay); the layer's number is the mask's site.
+``model.dropout_seed`` where that is set (a one-element int64 tensor on the device; a captured
+training step needs it, to draw new masks on replay); the layer's number is the mask's site.
 """
 from typing import List, Optional, Tuple
 
@@ -136,6 +136,9 @@ class NGCF(BaseRecommender):
             return None
         if self.dropout_seed is not None:
             return self.dropout_seed
+        if self.user_embedding.weight.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("NGCF: a captured step needs model.dropout_seed (an int64 tensor "
+                               "on the device); a seed drawn now would be every replay's")
         return int(torch.randint(0, 2 ** 63 - 1, (1,)).item())
 
     def forward(self, adj_matrix) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -63,3 +63,29 @@ def test_masks_are_drawn_where_a_layer_drops(cuda, kw):
     m.layers[0].dropout.p = 0.5
     m.dropout = 0.0
     assert not torch.equal(torch.cat(m(g)), torch.cat(m(g)))
+
+
+def test_a_captured_step_needs_a_seed_on_the_device(cuda):
+    """A seed drawn on the host would be every replay's."""
+    g, _ = _graph()
+    g = g.to(cuda)
+    m = _model(counter_dropout=True).to(cuda).train()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        m(g)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.no_grad():
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            with pytest.raises(RuntimeError, match="dropout_seed"):
+                m(g)
+            kept = torch.zeros(4, device=cuda).add_(1)      # the capture itself goes on
+        m.eval()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):                       # nothing is drawn: no seed needed
+            out = torch.cat(m(g))
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, torch.cat(m(g)))
+    del kept
