@@ -185,8 +185,8 @@ inline bool make_drop(Drop* d, const char* what, double p, uint64_t seed, const 
     set_error("%s: p must be between 0 and 1, got %g", what, p);
     return false;
   }
-  if (row0 < 0) {
-    set_error("%s: negative row0", what);
+  if (row0 < 0 || row0 > (int64_t)1 << 62) {  // row0 + row stays within 63 bits
+    set_error("%s: row0 must be between 0 and 2^62, got %lld", what, (long long)row0);
     return false;
   }
   const uint32_t border = (uint32_t)(p * 65536.0 + 0.5);

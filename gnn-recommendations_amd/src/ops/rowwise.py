@@ -153,8 +153,8 @@ def _drop_args(what: str, x: torch.Tensor, p: float, seed: Seed, site: int, row0
         raise ValueError(f"{what}: p must be between 0 and 1, got {p}")
     if not 0 <= int(site) < 2 ** 32:
         raise ValueError(f"{what}: site must be a 32-bit number, got {site}")
-    if int(row0) < 0:
-        raise ValueError(f"{what}: row0 must not be negative, got {row0}")
+    if not 0 <= int(row0) <= 2 ** 62:
+        raise ValueError(f"{what}: row0 must be between 0 and 2^62, got {row0}")
     tensor = None
     if isinstance(seed, torch.Tensor):
         if seed.numel() != 1 or seed.dtype != torch.int64:

@@ -641,10 +641,11 @@ int gnnrec_adam_step_f32(float* param, const float* grad, float* exp_avg, float*
  * the activation; slope 1: no activation), from a counter-based generator instead of a stored
  * mask. A value is dropped when its 16-bit draw is below round(p * 65536) (p in [0, 1]) and
  * scaled by 65536 / (65536 - round(p * 65536)) otherwise. The draws are Philox4x32-10 with key =
- * seed and counter = (column / 8, row0 + row, site), eight columns a block, so a value's fate
- * depends on its place alone and the backward pass draws it again. seed_ptr, if not NULL, is a
- * device int64 read instead of `seed` (a captured graph then replays with new masks). A dropped
- * value is 0 whatever the input holds there. `site` tells the dropouts of one step apart.
+ * seed and counter = (column / 8, row0 + row, site), eight columns a block (row0 from 0 to 2^62),
+ * so a value's fate depends on its place alone and the backward pass draws it again. seed_ptr, if
+ * not NULL, is a device int64 read instead of `seed` (a captured graph then replays with new
+ * masks). A dropped value is 0 whatever the input holds there. `site` tells the dropouts of one
+ * step apart.
  *   forward : y  = keep ? act(x) * s : 0
  *   backward: dx = keep ? dy * s * act'(x) : 0     (x may be NULL when slope == 1) */
 int gnnrec_dropout_forward(int32_t dtype, int64_t rows, int64_t d, const void* x, int64_t ldx,

@@ -9,7 +9,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
 from src import ops
-from src.ops import q4, rowwise
+from src.ops import _lib, q4, rowwise
 
 
 @pytest.fixture
@@ -111,3 +111,19 @@ def test_tracing_is_refused_on_the_device(cuda, call):
     _traces(cuda, {"q4_matmul": lambda x: ops.q4_matmul(x, table),
                    "quantize_q4": lambda x: ops.quantize_q4(x).scale,
                    "dequantize": lambda x: table.dequantize() + x.detach()[:3]}.get(call) or CALLS[call])
+
+
+def test_row0_past_64_bits_is_refused(stand_in):
+    """A C entry would see it modulo 2^64: another row's draws. The bound leaves room for the
+    rows behind it."""
+    x = torch.ones(4, 8)
+    for row0 in (2 ** 62 + 1, 2 ** 63, 2 ** 64, 2 ** 64 + 5):
+        for call in (lambda: ops.dropout(x, 0.1, 1, row0=row0),
+                     lambda: ops.dropout_add_layer_norm(x, x, None, None, 0.1, 1, row0=row0)):
+            with pytest.raises(ValueError, match="row0"):
+                call()
+    assert ops.dropout(x, 0.1, 1, row0=2 ** 62).shape == (4, 8)
+    L, a = _lib.lib(), x.data_ptr()
+    assert L.gnnrec_dropout_forward(0, 4, 8, a, 8, a, 8, 0.1, 1, None, 0, 2 ** 62 + 1, 1.0,
+                                    None) == -1
+    assert "row0" in L.gnnrec_last_error().decode()
