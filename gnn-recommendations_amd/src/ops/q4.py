@@ -16,7 +16,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .rowwise import launch, ptr, rows_of
+from ._lib import ptr
+from .rowwise import launch, rows_of
 
 GROUP = 32     # columns that share a scale; the kernels' matrix step is as deep
 SHORT_COLUMNS = 256     # up to here the users need no workspace (csrc/q4.hip plan_of)
@@ -129,6 +130,7 @@ def q4_matmul(x: torch.Tensor, table: Q4Table,
     if k > SHORT_COLUMNS:
         nbytes = _lib.lib().gnnrec_q4_matmul_work_bytes(t, m, n, k)
         work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    launch("gnnrec_q4_matmul", device, t, _lib.DTYPES[out_dtype], m, ptr(x2), x2.stride(0),
-           n, k, ptr(codes), ptr(table.scale), ptr(out), n, ptr(work))
+    launch("gnnrec_q4_matmul", device, t, _lib.DTYPES[out_dtype], m, x2.data_ptr(),
+           x2.stride(0), n, k, codes.data_ptr(), table.scale.data_ptr(), out.data_ptr(), n,
+           ptr(work))
     return out

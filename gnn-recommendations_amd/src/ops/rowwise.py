@@ -35,9 +35,10 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx import _symbolic_trace as _fx_trace
 
 from . import _lib
-from ._lib import check
+from ._lib import check, ptr
 
 MAX_NORM_WIDTH = 16384    # csrc/layer_norm.hip kNormMaxD
 
@@ -51,15 +52,18 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-_jit_tracing = torch._C._get_tracing_state
+_jit_tracing = torch._C._is_tracing
 _modes = torch._C._len_torch_dispatch_stack
-_pre_dispatch_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
+_transform = torch._C._functorch.peek_interpreter_stack
 
 
 def _refuse_tracing(name: str) -> None:
-    """Raise if a graph is being recorded (and not if another dispatch mode is active)."""
+    """Raise if a graph is being recorded or tensors are functionalize's wrappers, which have no
+    address (and not under another mode or transform)."""
     from torch.fx.experimental.proxy_tensor import get_proxy_mode
-    if _jit_tracing() is not None or get_proxy_mode() is not None:
+    functionalize = torch._C._functorch.TransformType.Functionalize
+    if _jit_tracing() or get_proxy_mode() is not None or any(
+            t.key() == functionalize for t in torch._C._functorch.get_interpreter_stack() or ()):
         raise RuntimeError(f"{name}: cannot be traced; a recorded graph would hold the result's "
                            "allocation without the launch that fills it, and this call's sizes")
 
@@ -68,7 +72,7 @@ def launch(name: str, device: torch.device, *args) -> None:
     """Call a C entry on `device`'s current stream, whatever device is current; refused while
     torch.jit.trace or make_fx records. The calls of a small table cost the host more than the
     GPU, so nothing is looked up twice here."""
-    if _jit_tracing() is not None or _modes() or _pre_dispatch_modes():
+    if _jit_tracing() or _fx_trace._is_fx_tracing_flag or _modes() or _transform() is not None:
         _refuse_tracing(name)
     fn = _ENTRIES.get(name)
     if fn is None:
@@ -81,18 +85,6 @@ def launch(name: str, device: torch.device, *args) -> None:
             rc = fn(*args, _raw_stream(i))
     if rc:
         check(rc, name)
-
-
-def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    """t's address, None for no tensor. One without memory of its own (functionalize's wrappers)
-    is refused: its address reads as NULL, which to a C entry is an absent table."""
-    if t is None:
-        return None
-    address = t.data_ptr()
-    if not address and t.numel():
-        raise RuntimeError(f"the row-wise operators need tensors in memory, got {type(t).__name__} "
-                           f"{tuple(t.shape)} without an address")
-    return address
 
 
 def rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -196,8 +188,8 @@ def _dropout_forward(x, ldx, rows, mask):
     seed_t, pre, post = mask
     y = _empty_rows(x)
     d = x.shape[-1]
-    launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, ptr(x), ldx,
-           ptr(y), d, *pre, ptr(seed_t), *post)
+    launch("gnnrec_dropout_forward", x.device, _lib.DTYPES[x.dtype], rows, d, x.data_ptr(), ldx,
+           y.data_ptr(), d, *pre, ptr(seed_t), *post)
     return y
 
 
@@ -208,7 +200,7 @@ def _dropout_backward(x, dy, rows, mask):
     dx = _empty_rows(dy)
     d = dy.shape[-1]
     launch("gnnrec_dropout_backward", dy.device, _lib.DTYPES[dy.dtype], rows, d, ptr(x), ldx,
-           ptr(dy), lddy, ptr(dx), d, *pre, ptr(seed_t), *post)
+           dy.data_ptr(), lddy, dx.data_ptr(), d, *pre, ptr(seed_t), *post)
     return dx
 
 
@@ -246,8 +238,8 @@ def _norm_forward(x, res, w, b, cfg):
     y = _empty_rows(x)
     h = torch.empty_like(y) if keep_h else None
     d = x.shape[-1]
-    launch("gnnrec_layer_norm_forward", x.device, t, wt, rows, d, ptr(x), ldx, ptr(res), ldr,
-           ptr(w), ptr(b), eps, *pre, ptr(seed_t), *post, ptr(y), d, ptr(h), d)
+    launch("gnnrec_layer_norm_forward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res), ldr,
+           ptr(w), ptr(b), eps, *pre, ptr(seed_t), *post, y.data_ptr(), d, ptr(h), d)
     return y, h
 
 
@@ -285,8 +277,8 @@ class _NormBlock(torch.autograd.Function):
         work = None
         if need_w or need_b:
             work = x.new_empty(_norm_work_floats(rows, d), dtype=torch.float32)
-        launch("gnnrec_layer_norm_backward", x.device, t, wt, rows, d, ptr(x), ldx, ptr(res),
-               ldr, ptr(w), eps, *pre, ptr(seed_t), *post, ptr(dy), lddy, ptr(dh), lddh,
+        launch("gnnrec_layer_norm_backward", x.device, t, wt, rows, d, x.data_ptr(), ldx, ptr(res),
+               ldr, ptr(w), eps, *pre, ptr(seed_t), *post, dy.data_ptr(), lddy, ptr(dh), lddh,
                ptr(dx), d, ptr(dres), d, ptr(dw), ptr(db), ptr(work))
         return dx, dres, dw, db, None
 
