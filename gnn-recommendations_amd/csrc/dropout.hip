@@ -8,8 +8,8 @@
 // holds there, infinities and NaN included.
 //
 // One thread takes one block of eight columns: one Philox block, 16-B accesses. Bound by memory:
-// 2M x 64 fp32 forward 171 us (6.0 TB/s; a copy of that size reaches 5.0 to 5.3), backward 266 us
-// (5.8); 65 537 x 321 bf16, rows of odd width and no alignment, 21 us each (4.0).
+// 2M x 64 fp32 forward 176 us (5.8 TB/s; torch's copy of 2 GiB reaches 4.9), backward 264 us (5.8);
+// 65 537 x 321 bf16, rows of odd width and no alignment, 21 us each (4.0).
 #include "rowwise.h"
 
 namespace gnnrec {

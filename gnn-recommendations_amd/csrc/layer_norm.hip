@@ -18,10 +18,15 @@
 // writes one partial row; a second launch adds the partial rows, each column in a fixed order
 // (no atomics: equal inputs give equal bits).
 //
-// fp32 tables are bound by memory (the block on 2M x 64: forward 187 us, 5.5 TB/s, backward 302 us,
-// 5.1, sums 4 us), wide half-precision rows too (8192 x 4096 bf16 alone: 30, 44 and 5 us);
-// half-precision blocks by instructions, most of them the generator's and the conversions' (100 003
-// x 201 fp16: 38, 60 and 4 us, the VALU busy in 64 and 62 % of the cycles).
+// fp32 tables are bound by memory (the block on 2M x 64: forward 373 us, 5.5 TB/s, backward 601 us,
+// 5.1, sums 5 us), wide half-precision rows too (8192 x 4096 bf16 alone: 30, 44 and 5 us). A
+// half-precision block is short of both limits (100 003 x 201 fp16: 39, 62 and 4 us, 4.1 and 3.9
+// TB/s with the VALU busy in 64 and 62 % of the cycles, most of it the generator's and the
+// conversions' instructions). A width just above one that fills its lanes takes twice as many:
+// 8192 x 4097 fp16, both passes, 172 us, 4096 columns 80.
+//
+// Deviations are squared in fp32: a row whose squares add up to more than it holds (64 deviations of
+// 2.4e18) comes out as the bias.
 #include <type_traits>
 
 #include "rowwise.h"

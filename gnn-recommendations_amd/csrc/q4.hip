@@ -7,9 +7,12 @@
 //   out[i, r]   = sum over groups g of scale[r, g] * (sum over c in g of x[i, c] e2m1(code[r, c]))
 // E2M1 is the 4-bit type that this hardware converts by itself (two codes an instruction).
 //
-// All of it is bound by the table's bytes: one user against 1M x 64 9.6 us (4.2 TB/s), 16 users
-// against 1M x 256 bf16 48 us (3.7), 8192 x 8192 and one user 13.7 us (2.8: latency of
-// rounds of loads); the quantiser 1M x 64 fp32 66 us (4.4).
+// Short rows are bound by the table's bytes: one user against 1M x 64 9.7 us (36 MB, which may lie
+// in the 256 MB cache: 4.1 TB/s), 16 users against 1M x 256 bf16 48 us (3.7). Long rows are not:
+// 8192 x 8192 and one user 13.4 us (2.8: each round of loads waits for the one before to be
+// multiplied), 16 fp32 users 35 us (1.1: the users' fragments from the caches, see q4_many_kernel).
+// The quantiser: 1M x 64 fp32 68 us (4.3, the VALU busy in 76 % of the cycles), bf16 59 (2.8, 86 %:
+// instructions, seven comparisons a value among them).
 #include <type_traits>
 
 #include "rowwise.h"
@@ -465,6 +468,9 @@ __global__ __launch_bounds__(WK * 64, 4) void q4_few_kernel(const T* __restrict_
 // Long rows, more users: they come as bf16 parts in rows of whole groups (plane i at x + i *
 // plane, rows ldx apart), from the table itself or from split_users_kernel, and a step's
 // fragments (1 KB a group and part) are loaded from the caches with its codes, one step ahead.
+// The waves split the groups, so each fragment is loaded once for every 32 (64) items: 16 fp32
+// users x 8192 x 8192 move 200 MB of them beside 38 MB of codes, with one wave a SIMD resident (256
+// workgroups of four), in 35 us; bf16 users, a third of the fragments, in 19.
 template <int PARTS, int NT, int WK>
 __global__ __launch_bounds__(WK * 64, 2) void q4_many_kernel(const bf16_t* __restrict__ x,
                                                           int64_t ldx, int64_t plane, Q4Args p) {
@@ -612,10 +618,11 @@ static int run_few(int32_t dtype, const T* x, int64_t ldx, const Q4Args& p, hipS
   return p.ng >= 64 ? go(i1, i8, i2) : go(i1, i4, i2);
 }
 
-// Two tiles a wave set: 16 users x 8192 x 8192 fp32 35.3 us (eight waves 36.3), x 2000 x 1000 9.6
-// (four tiles 12.2), x 20 000 x 3100 bf16 20.2 (four tiles 22.4). Four where there are several
-// user tiles and many items, so that a fragment serves more of them: 64 users x 7812 x 8192 82 us
-// (two 120), x 10 000 x 1000 23.4 (25.6); but x 300 x 3000 22.2 (17.3).
+// Two tiles a wave set: 16 users x 8192 x 8192 fp32 35.2 us (eight waves 36.3), x 2000 x 1000 fp32
+// 9.5 (four tiles 12.2), x 20 000 x 3100 bf16 20.1 (four tiles 22.4). Four where there are several
+// user tiles and many items, so that a fragment serves more of them: 64 users x 7812 x 8192 fp32
+// 82.6 us (two 120; bf16 48.5), x 10 000 x 1000 fp32 23.5 (25.6); but x 300 x 3000 fp32 22.2
+// (17.4).
 template <int PARTS>
 static int run_many(const bf16_t* x, int64_t ldx, int64_t plane, const Q4Args& p,
                     hipStream_t stream) {

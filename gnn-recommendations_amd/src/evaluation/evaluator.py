@@ -133,9 +133,10 @@ def embedding_statistics(emb, exact_limit: int = 65536, chunk: int = 4096,
 
 
 class Evaluator:
-    """item_bits = 4 ranks against the item table in 4 bits (ops.quantize_q4), as a server that
-    holds it so would answer: the metrics then tell what that table costs in quality. The same
-    order and masking; needs a ROCm device."""
+    """item_bits = 4 ranks by the scores of the item table in 4 bits (ops.quantize_q4): the metrics
+    then tell what that table costs in quality (not in time: every user's scores are sorted
+    whole). Order, masking and places without an item are the fp32 ranking's; needs a ROCm
+    device."""
 
     def __init__(self, k_values=(10, 20), device: Optional[torch.device] = None,
                  item_bits: int = 32):

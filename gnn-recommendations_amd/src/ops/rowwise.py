@@ -323,7 +323,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     """(x - mean) / sqrt(var + eps) * weight + bias over x's last dimension (at most
     MAX_NORM_WIDTH values; var divides by their number). weight and bias: x's dtype or float32,
     either may be None. Gradients of x, weight and bias; the weight's and the bias's are summed
-    over all rows in fp32 in a fixed order."""
+    over all rows in fp32 in a fixed order. Deviations are squared in fp32: a row whose squares
+    add up to more than it holds (64 deviations of 2.4e18) comes out as the bias."""
     return _norm_block("layer_norm", False, x, None, weight, bias, eps, _NO_MASK)[0]
 
 

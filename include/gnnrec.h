@@ -635,7 +635,9 @@ int gnnrec_adam_step_f32(float* param, const float* grad, float* exp_avg, float*
 
 /* ---- row-wise operators of the training path ---------------------------------------------
  * Tables of `rows` rows of d values (dtype: gnnrec_dtype), leading dimensions in elements (0 is
- * allowed for an input: one row for all). 32-bit arithmetic, one rounding at the store.
+ * allowed for an input: one row for all). No output may overlap an input or another output: a
+ * row's last, partial eight is read together with its neighbour's columns. 32-bit arithmetic, one
+ * rounding at the store.
  *
  * Dropout with a LeakyReLU in front, as NGCF's layers end (baselines/ngcf.py:84-86: dropout of
  * the activation; slope 1: no activation), from a counter-based generator instead of a stored
