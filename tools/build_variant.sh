@@ -7,9 +7,12 @@ OUT=$1; SRC=$2; shift 2
 B=gnn-recommendations_amd/build
 mkdir -p "$(dirname "$OUT")"
 T=$(mktemp -d)
-/opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -fPIC -std=c++17 -ffp-contract=off \
-  -fhip-fp32-correctly-rounded-divide-sqrt "$@" -c "gnn-recommendations_amd/csrc/$SRC" -o "$T/v.o"
+HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
+# the library's own flags: a variant differs from it by its -D flags alone
+FLAGS=$(PYTHONPATH=gnn-recommendations_amd python3 -c \
+  'import build_native; print(*build_native.CFLAGS)')
+$HIPCC $FLAGS "$@" -c "gnn-recommendations_amd/csrc/$SRC" -o "$T/v.o"
 OBJS=$(ls $B/*.o | grep -v "/$SRC.o$")
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o "$OUT" $OBJS "$T/v.o" -lpthread
+$HIPCC --offload-arch=gfx950 -shared -fPIC -o "$OUT" $OBJS "$T/v.o" -lpthread
 rm -rf "$T"
 echo "$OUT"

@@ -1,7 +1,8 @@
 // Dependent fp32 FMA chain latency on gfx950, one wave: cycles per fmaf of a chain of N
 // dependent v_fma_f32 (the heavy-row consumer's per-neighbour floor), for 1, 2
 // and 4 interleaved independent chains per lane, and with a ds_read_b32 feeding each fmaf.
-//   hipcc -O3 --offload-arch=gfx950 -ffp-contract=off tools/fma_latency.hip -o tools/bin/fma_latency
+//   hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops
+//       tools/fma_latency.hip -o tools/bin/fma_latency
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

@@ -6,7 +6,8 @@
 //  MFMA: the same [32 x 64] x [64 x 4 -> padded 16] product as v_mfma_f32_16x16x4_f32 (2 M tiles
 //        x 16 K steps = 32 MFMAs), the operands already in MFMA fragment layout — a lower bound
 //        for the matrix-core form (it also needs the rows transposed through LDS).
-//   hipcc -O3 --offload-arch=gfx950 -ffp-contract=off tools/gat_score_mfma.hip -o gat_score_mfma
+//   hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops
+//       tools/gat_score_mfma.hip -o gat_score_mfma
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

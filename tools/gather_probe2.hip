@@ -4,7 +4,8 @@
 // buffer resource with 32-bit offsets as the hop does. Each wave keeps two batches of DEPTH
 // instructions in flight (batch b+1 issued before batch b is consumed), 16 waves per CU, one
 // 1024-thread workgroup per CU. Tables: power-of-two sizes so the line index is a mask.
-//   hipcc --offload-arch=gfx950 -O3 tools/gather_probe2.hip -o tools/_var/gather_probe2
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops
+//       tools/gather_probe2.hip -o tools/_var/gather_probe2
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -4,7 +4,8 @@
 // resource with 32-bit offsets. Two batches of DEPTH instructions in flight per wave, 16 waves
 // per CU. Question: is the beyond-L2 path limited by requests (a 64-B sector costs a 128-B
 // line's slot) or by bytes?
-//   hipcc --offload-arch=gfx950 -O3 tools/gather_probe3.hip -o tools/_var/gather_probe3
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops
+//       tools/gather_probe3.hip -o tools/_var/gather_probe3
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
