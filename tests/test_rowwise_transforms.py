@@ -127,3 +127,33 @@ def test_row0_past_64_bits_is_refused(stand_in):
     assert L.gnnrec_dropout_forward(0, 4, 8, a, 8, a, 8, 0.1, 1, None, 0, 2 ** 62 + 1, 1.0,
                                     None) == -1
     assert "row0" in L.gnnrec_last_error().decode()
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_export_is_refused(stand_in, call):
+    class Module(torch.nn.Module):
+        def forward(self, x):
+            return CALLS[call](x)
+
+    with pytest.raises(RuntimeError):
+        torch.export.export(Module(), (torch.ones(4, 8),), strict=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", [*CALLS, "q4_matmul"])
+def test_compiled_functions_run_the_operators(cuda, call):
+    """A call runs between the compiled parts, for other sizes and in the backward pass too."""
+    table = _table(cuda)
+    op = CALLS.get(call) or (lambda x: ops.q4_matmul(x.detach(), table))
+
+    def both(x):
+        return op(x * 2.0) + 1.0
+
+    compiled = torch.compile(both, backend="eager")
+    for rows in (4, 9):
+        x = torch.randn(rows, 8, device=cuda, requires_grad=True)
+        y, z = both(x), compiled(x)
+        assert torch.equal(y, z)
+        if y.requires_grad:
+            g = torch.randn_like(y)
+            assert torch.equal(torch.autograd.grad(y, x, g)[0], torch.autograd.grad(z, x, g)[0])
