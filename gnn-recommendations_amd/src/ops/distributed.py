@@ -516,7 +516,7 @@ def ngcf_forward_dist(dg: DistributedGraph, model, x0_pad: torch.Tensor, *,
     x_in = x0_pad
     for k, (layer, gs) in enumerate(zip(model.layers, gs_layers)):
         y = local[:, c0:c0 + widths[k + 1]]
-        if layer.norm is None:
+        if getattr(layer, "norm", None) is None:
             layer_fn(dg.shard, x_in, x_local, layer, gs, y)
         else:    # the norm is row-local, between the layer and its Group-and-Shuffle transform
             layer_fn(dg.shard, x_in, x_local, layer, None, y)
