@@ -141,14 +141,19 @@ class NGCF(BaseRecommender):
                                "on the device); a seed drawn now would be every replay's")
         return int(torch.randint(0, 2 ** 63 - 1, (1,)).item())
 
+    def _mask_arguments(self):
+        """What each layer is told of its mask; nothing where none is drawn."""
+        seed = self._mask_seed()
+        return [{} if seed is None else {"seed": seed, "site": k} for k in range(len(self.layers))]
+
     def forward(self, adj_matrix) -> Tuple[torch.Tensor, torch.Tensor]:
         x_final = self._native_concat_forward(adj_matrix, [None] * self.n_layers)
         if x_final is None:
             x = self._initial_table()
             outs = [x]
-            seed = self._mask_seed()
-            for k, layer in enumerate(self.layers):
-                x = layer(x, adj_matrix, seed=seed, site=k)
+            mask = self._mask_arguments()
+            for layer, kw in zip(self.layers, mask):
+                x = layer(x, adj_matrix, **kw)
                 outs.append(x)
             x_final = torch.cat(outs, dim=1)
         user_emb, item_emb = torch.split(x_final, [self.n_users, self.n_items], dim=0)
@@ -216,9 +221,9 @@ class NGCFGroupShuffle(NGCF):
         if x_final is None:
             x = self._initial_table()
             outs = [x]
-            seed = self._mask_seed()
-            for k, (layer, gs) in enumerate(zip(self.layers, self.gs_layers)):
-                x = layer(x, adj_matrix, gas=gs, seed=seed, site=k)
+            mask = self._mask_arguments()
+            for layer, gs, kw in zip(self.layers, self.gs_layers, mask):
+                x = layer(x, adj_matrix, gas=gs, **kw)
                 outs.append(x)
             x_final = torch.cat(outs, dim=1)
         user_emb, item_emb = torch.split(x_final, [self.n_users, self.n_items], dim=0)
