@@ -43,6 +43,13 @@ class NGCFLayer(nn.Module):
         self.norm = nn.LayerNorm(out_dim) if layer_norm else None
         self.single_kernel = False  # True: gather + MFMA in one launch (see ops.ngcf_layer)
 
+    def __setstate__(self, state):
+        """A layer that was saved whole before it had the options is one without them."""
+        super().__setstate__(state)
+        self.__dict__.setdefault("counter_dropout", False)
+        if not hasattr(self, "norm"):
+            self.norm = None
+
     def _fused_ok(self, x: torch.Tensor, a) -> bool:
         return (isinstance(a, CsrGraph) and not (torch.is_grad_enabled() and (
             x.requires_grad or self.W1.weight.requires_grad))
@@ -99,6 +106,8 @@ class NGCFLayer(nn.Module):
 
 
 class NGCF(BaseRecommender):
+    dropout_seed: Optional[torch.Tensor] = None     # see the module's text
+
     def __init__(self, n_users: int, n_items: int, embedding_dim: int = 64,
                  layer_sizes: Optional[List[int]] = None, dropout: float = 0.1,
                  init_scale: float = 0.01, counter_dropout: bool = False,
@@ -115,7 +124,6 @@ class NGCF(BaseRecommender):
         self.layers = nn.ModuleList(NGCFLayer(dims[k], dims[k + 1], dropout, counter_dropout,
                                               layer_norm)
                                     for k in range(self.n_layers))
-        self.dropout_seed: Optional[torch.Tensor] = None
         self.reset_parameters()
 
     def reset_parameters(self):

@@ -1,4 +1,6 @@
-"""NGCF over layers of the caller's own."""
+"""NGCF layers and models made before their row-wise options, or by the caller."""
+import copy
+
 import pytest
 import torch
 
@@ -29,3 +31,30 @@ def test_layers_with_the_former_arguments(cls):
             m.layers[k] = own
         for mode in (False, True):
             assert torch.equal(torch.cat(m.train(mode)(adj)), want)
+
+
+@pytest.mark.parametrize("cls", [NGCF, NGCFGroupShuffle])
+def test_models_made_before_the_options(cls):
+    """A model object that was saved whole has none of the options' attributes."""
+    m = _model(cls).eval()
+    adj, _, _ = torch_adj()
+    state = copy.deepcopy(m.__dict__)
+    state.pop("dropout_seed", None)
+    for layer in state["_modules"]["layers"]:
+        layer.__dict__.pop("counter_dropout")
+        layer.__dict__.pop("norm", None)
+        layer._modules.pop("norm", None)
+    old = cls.__new__(cls)
+    for k, layer in enumerate(state["_modules"]["layers"]):
+        again = NGCFLayer.__new__(NGCFLayer)
+        again.__setstate__(layer.__dict__)
+        state["_modules"]["layers"][k] = again
+    old.__setstate__(state)
+    with torch.no_grad():
+        assert torch.equal(torch.cat(old(adj)), torch.cat(m(adj)))
+    torch.manual_seed(3)
+    want = torch.cat(m.train()(adj))
+    torch.manual_seed(3)
+    assert torch.equal(torch.cat(old.train()(adj)), want)
+    new = copy.deepcopy(_model(cls, layer_norm=True, counter_dropout=True))
+    assert all(layer.norm is not None and layer.counter_dropout for layer in new.layers)
